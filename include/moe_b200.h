@@ -762,6 +762,50 @@ int moe_sample_tokens(const float *logits, int T, int V, float temperature, floa
                       uint64_t counter, int32_t *ids, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * Log-probabilities of rows of logits [T, V] fp32 (4-byte aligned, any V): with
+ * lse = log sum_v exp(l_v),
+ *   logprob[t]       = l[targets[t]] - lse; NaN where targets[t] is -1 (no token given). Another id
+ *                      outside [0, V) gives NaN and sets bit 2 of the device error word. targets
+ *                      and logprob are both NULL when no tokens are given.
+ *   entropy[t]       = lse - sum_v p_v l_v, in nats
+ *   top_ids[t][i], top_logprobs[t][i], i < n: the n largest logits (equal ones: the lower id
+ *                      first; a NaN orders as -inf) and their log-probabilities; 0 <= n <= min(V, 32)
+ * A logit of -inf is a masked token. A row that holds a NaN or +inf, or nothing above -inf, has no
+ * distribution: its log-probabilities and entropy are NaN, its ids are still in order. One launch,
+ * no workspace; the results do not depend on the other rows of the call up to rounding.
+ */
+int moe_token_logprobs(const float *logits, int T, int V, const int32_t *targets, int n, float *logprob,
+                       float *entropy, int32_t *top_ids, float *top_logprobs, void *stream);
+
+/* Bytes of workspace moe_head_logprobs needs; it need not be zeroed and holds nothing between calls. */
+size_t moe_head_logprobs_workspace_bytes(int T, int V, int n);
+
+/*
+ * The same outputs straight from bf16 rows x [T, H] and the bf16 head [V, H] (both 16-byte aligned,
+ * H a multiple of 8 up to 8192; any T): prompt scoring without [T, V] logits in memory. The ids are
+ * in the order of the logits moe_lm_head_logits computes. Calls that share a workspace must not
+ * overlap on the GPU.
+ */
+int moe_head_logprobs(const void *head, int V, int H, const void *x, int T, const int32_t *targets, int n,
+                      float *logprob, float *entropy, int32_t *top_ids, float *top_logprobs, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------ */
+/* Low-rank adapters of many requests beside a shared projection                          */
+/* ------------------------------------------------------------------------------------ */
+
+/*
+ * out[t] = y[t] + scale[a] * (x[t] . A[a]^T) . B[a]^T with a = ids[t], for rows x [T, K] bf16 and the
+ * shared projection's outputs y [T, N] (bf16, or fp32 logits with y_fp32 = 1). A [adapters, rank, K]
+ * and B [adapters, N, rank] bf16, scale [adapters] fp32, ids [T] int32 on the device, in any order.
+ * ids[t] = -1 copies the row; another id outside [0, adapters) copies it too and sets bit 2 of the
+ * device error word. Sums are fp32, rounded once to y's type. K and rank are multiples of 8, rank at
+ * most 128; x, A and B 16-byte aligned; out may be y itself but overlap nothing else.
+ */
+int moe_adapter_add(const void *x, int T, int K, int N, const void *a, const void *b, const float *scale,
+                    int adapters, int rank, const int32_t *ids, const void *y, int y_fp32, void *out, void *stream);
+
+/*
  * Device-side error word (bit 1: a bounded mbarrier/flag wait gave up, bit 2: invalid
  * input seen by a kernel, bit 4: an expert-parallel peer did not signal within 2 s). Returns the current value (>= 0) and clears it when `clear`.
  * Kernels never trap: they record the condition here and skip the affected work.

@@ -45,6 +45,10 @@ SIGNATURES: dict[str, tuple] = {
     "moe_lm_head_argmax": (I, [P, I, I, P, I, P, P, P, SZ, P]),
     "moe_sample_workspace_bytes": (SZ, [I, I]),
     "moe_sample_tokens": (I, [P, I, I, ctypes.c_float, ctypes.c_float, U64, U64, P, P, SZ, P]),
+    "moe_token_logprobs": (I, [P, I, I, P, I, P, P, P, P, P]),
+    "moe_head_logprobs_workspace_bytes": (SZ, [I, I, I]),
+    "moe_head_logprobs": (I, [P, I, I, P, I, P, I, P, P, P, P, P, SZ, P]),
+    "moe_adapter_add": (I, [P, I, I, I, P, P, P, I, I, P, P, I, P, P]),
     "moe_experts_gateup": (I, [P, I, I, I, I, I, P, P, P, P, P, P, P, I, I, I, P, P]),
     "moe_experts_down": (I, [P, I, I, I, I, I, P, P, P, P, P, I, I, I, P, P, P, P, P]),
     "moe_device_error": (I, [I]),

@@ -1,0 +1,147 @@
+// Row statistics of a softmax and the n largest entries of a row, as the log-probability
+// kernels (logprobs.cu, headscore.cu) keep them.
+#pragma once
+
+#include "common.cuh"
+
+constexpr int kTopMax = 32;            // alternatives a row can be asked for: one per lane of a warp
+
+// Softmax statistics over a set of values x: m the largest, s = sum e^(x - m) over the set
+// WITHOUT one occurrence of m, w = sum (x - m) e^(x - m). Keeping the largest out of s keeps the
+// digits of rows whose probability is all but one: lse - m = log1p(s), and s itself is then far
+// below the rounding of 1 + s. Nothing yet: m = -inf. A NaN among the values ends up in s; a row
+// whose m is not finite has no distribution (soft_log_rest is NaN).
+struct Soft {
+    float m, s, w;
+};
+
+// e^kSoftFar is 0 in fp32: differences are held above it, so that 0 x inf does not arise for masked
+// (-inf) or lowest-value logits
+constexpr float kSoftFar = -1000.f;
+
+MOE_D Soft soft_none() { return Soft{-INFINITY, 0.f, 0.f}; }
+
+MOE_D Soft soft_merge(Soft a, Soft b) {
+    if (a.m < b.m) { const Soft t = a; a = b; b = t; }
+    if (b.m == -INFINITY) {                      // nothing there (s is 0, or NaN to be passed on)
+        a.s += b.s;
+        return a;
+    }
+    const float d = fmaxf(b.m - a.m, kSoftFar), e = __expf(d);
+    a.w += e * (b.w + d * (b.s + 1.f));
+    a.s += (b.s + 1.f) * e;
+    return a;
+}
+
+// lse - m, NaN for a row without a distribution
+MOE_D float soft_log_rest(const Soft &a) {
+    return (a.m < INFINITY && a.m > -INFINITY) ? log1pf(a.s) : __int_as_float(0x7fffffff);
+}
+
+// entropy in nats: lse - sum p x = log1p(s) - w / (1 + s)
+MOE_D float soft_entropy(const Soft &a) { return soft_log_rest(a) - a.w / (1.f + a.s); }
+
+MOE_D Soft soft_shfl_xor(const Soft &a, int off) {
+    return Soft{__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.s, off),
+                __shfl_xor_sync(0xffffffffu, a.w, off)};
+}
+
+MOE_D Soft soft_warp(Soft a) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        const Soft b = soft_shfl_xor(a, off);
+        // both lanes of a pair merge in the same order, so that every lane ends with the same bits
+        a = (threadIdx.x & off) ? soft_merge(b, a) : soft_merge(a, b);
+    }
+    return a;
+}
+
+// Adds kN values (those with ok[i]) to a thread's statistics. at / idx: index of the thread's
+// first largest value; idx0 + i is the index of v[i]. NaN counts as -inf for the order.
+template <int kN>
+MOE_D void soft_add(Soft &a, int &at, const float (&v)[kN], int idx0) {
+    float cm = v[0];
+#pragma unroll
+    for (int i = 1; i < kN; ++i) cm = fmaxf(cm, v[i]);
+    int skip = -1;
+    if (cm > a.m) {                              // the old largest becomes one of the others
+        if (a.m == -INFINITY) {
+            a.w = 0.f;
+        } else {
+            const float d = fmaxf(a.m - cm, kSoftFar), e = __expf(d);
+            a.w = e * (a.w + d * (a.s + 1.f));
+            a.s = (a.s + 1.f) * e;
+        }
+        a.m = cm;
+#pragma unroll
+        for (int i = kN - 1; i >= 0; --i)
+            if (v[i] == cm) skip = i;
+        at = idx0 + skip;
+    }
+    if (a.m == -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (v[i] != v[i]) a.s = v[i];
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        const float d = v[i] - a.m;
+        const float e = i == skip ? 0.f : __expf(d);         // e^-inf = 0, NaN stays
+        a.s += e;
+        a.w += fmaxf(d, kSoftFar) * e;
+    }
+}
+
+// ------------------------------------------------------------------ order of the entries
+
+// Order-preserving 64-bit key of (value, index): larger value first, equal values the lower
+// index first. 0 is no entry. NaN orders as -inf, -0 as +0.
+MOE_D unsigned long long top_key(float v, int idx) {
+    v = v != v ? -INFINITY : v + 0.f;
+    const uint32_t u = __float_as_uint(v);
+    const uint32_t o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return ((unsigned long long)o << 32) | (unsigned long long)(0xffffffffu - (uint32_t)idx);
+}
+MOE_D float top_value(unsigned long long k) {
+    const uint32_t o = (uint32_t)(k >> 32);
+    return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+MOE_D int top_index(unsigned long long k) { return (int)(0xffffffffu - (uint32_t)(k & 0xffffffffull)); }
+
+// Bitonic networks over one key per lane, descending with the lane.
+MOE_D unsigned long long top_cmpx(unsigned long long k, int off, bool keep_max) {
+    const unsigned long long o = __shfl_xor_sync(0xffffffffu, k, off);
+    return (k > o) == keep_max ? k : o;
+}
+MOE_D unsigned long long top_sort(unsigned long long k) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int off = size >> 1; off > 0; off >>= 1)
+            k = top_cmpx(k, off, ((lane & off) == 0) == ((lane & size) == 0 || size == 32));
+    return k;
+}
+// a, b sorted descending over the lanes: the 32 largest of both, sorted descending
+MOE_D unsigned long long top_merge(unsigned long long a, unsigned long long b) {
+    const int lane = threadIdx.x & 31;
+    b = __shfl_sync(0xffffffffu, b, 31 - lane);
+    a = a > b ? a : b;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) a = top_cmpx(a, off, (lane & off) == 0);
+    return a;
+}
+// inserts the keys of the lanes in `who` (a warp-uniform mask) into a sorted list, one after another
+MOE_D unsigned long long top_insert(unsigned long long list, unsigned long long key, unsigned who) {
+    const int lane = threadIdx.x & 31;
+    while (who) {
+        const int src = __ffs(who) - 1;
+        who &= who - 1;
+        const unsigned long long k = __shfl_sync(0xffffffffu, key, src);
+        const unsigned long long up = __shfl_up_sync(0xffffffffu, list, 1);
+        // entries above k stay, the others move down by one, k takes the gap
+        if (list < k) list = (lane == 0 || up > k) ? k : up;
+    }
+    return list;
+}

@@ -8,6 +8,7 @@ Tensor conventions
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -25,6 +26,16 @@ def _ptr(t):
 def _stream(stream) -> int:
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
+
+
+def _launch_on(dev: torch.device, stream):
+    """Context under which a call on `dev` allocates and launches: the tensors' own device, which
+    need not be the current one, and `stream` when one is given."""
+    if stream is not None:
+        if stream.device != dev:
+            raise ValueError(f"stream is on {stream.device}, expected {dev}")
+        return torch.cuda.stream(stream)
+    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _need(t: torch.Tensor, name: str, dtypes, dev=None) -> None:

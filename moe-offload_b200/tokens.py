@@ -13,12 +13,76 @@ moe_lm_head_argmax for greedy steps, moe_lm_head_logits + moe_sample_tokens for 
 from __future__ import annotations
 
 import time
-from typing import Any, Iterable, Iterator
+from typing import Any, Iterable, Iterator, NamedTuple
 
 import torch
 
 from ._lib import call
-from .ops import _need, _stream
+from .ops import _launch_on, _need, _ptr, _stream
+
+MAX_ALTERNATIVES = 32
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row: the given token's log-probability (NaN where none was given), the entropy in nats,
+    and the ids and log-probabilities of the n most likely tokens (most likely first, equal ones
+    the lower id first). fp32 [T], fp32 [T], int32 [T, n], fp32 [T, n]."""
+
+    logprob: torch.Tensor | None
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def _logprob_outputs(T: int, V: int, targets: torch.Tensor | None, n: int, dev) -> TokenLogprobs:
+    if not 0 <= n <= min(V, MAX_ALTERNATIVES):
+        raise ValueError(f"{n} alternatives: 0 to {min(V, MAX_ALTERNATIVES)} can be asked for")
+    if targets is not None:
+        _need(targets, "targets", (torch.int32,), dev)
+        if targets.numel() != T:
+            raise ValueError(f"{targets.numel()} targets for {T} rows")
+    return TokenLogprobs(None if targets is None else torch.empty((T,), dtype=torch.float32, device=dev),
+                         torch.empty((T,), dtype=torch.float32, device=dev),
+                         torch.empty((T, n), dtype=torch.int32, device=dev),
+                         torch.empty((T, n), dtype=torch.float32, device=dev))
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, n: int = 0,
+                   stream=None) -> TokenLogprobs:
+    """logits fp32 [T, V], targets int32 [T] (-1: no token) -> TokenLogprobs. A logit of -inf is a
+    masked token; a row with a NaN, a +inf or nothing above -inf gives NaN."""
+    _need(logits, "logits", (torch.float32,))
+    if logits.dim() != 2:
+        raise ValueError(f"logits have shape {tuple(logits.shape)}, expected [T, V]")
+    T, V = logits.shape
+    dev = logits.device
+    with _launch_on(dev, stream):
+        r = _logprob_outputs(T, V, targets, n, dev)
+        if T:
+            call("moe_token_logprobs", logits.data_ptr(), T, V, _ptr(targets), n, _ptr(r.logprob),
+                 r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), _stream(stream))
+    return r
+
+
+def head_logprobs(head: torch.Tensor, h: torch.Tensor, targets: torch.Tensor | None = None, n: int = 0,
+                  stream=None) -> TokenLogprobs:
+    """token_logprobs of the logits of rows h bf16 [T, H] under the head bf16 [V, H], without the
+    [T, V] logits in memory (prompt scoring): any T."""
+    _need(head, "head", (torch.bfloat16,))
+    dev = head.device
+    _need(h, "h", (torch.bfloat16,), dev)
+    if head.dim() != 2 or h.dim() != 2 or h.shape[1] != head.shape[1]:
+        raise ValueError(f"rows {tuple(h.shape)} do not fit a head {tuple(head.shape)}")
+    V, H = head.shape
+    T = h.shape[0]
+    with _launch_on(dev, stream):
+        r = _logprob_outputs(T, V, targets, n, dev)
+        if T:
+            ws = torch.empty(int(call("moe_head_logprobs_workspace_bytes", T, V, n)), dtype=torch.uint8, device=dev)
+            call("moe_head_logprobs", head.data_ptr(), V, H, h.data_ptr(), T, _ptr(targets), n, _ptr(r.logprob),
+                 r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), ws.data_ptr(), ws.numel(),
+                 _stream(stream))
+    return r
 
 
 class ByteTokenizer:
@@ -102,6 +166,11 @@ class TokenHead:
              None if logits is None else logits.data_ptr(), out.data_ptr(), self._best.data_ptr(),
              self._best.numel() * 8, _stream(stream))
         return out
+
+    def score(self, h: torch.Tensor, targets: torch.Tensor | None = None, n: int = 0, stream=None) -> TokenLogprobs:
+        """h bf16 [T, H], targets int32 [T] -> TokenLogprobs under this head (head_logprobs)."""
+        _need(h, "h", (torch.bfloat16,), self.device)
+        return head_logprobs(self.head_w, h, targets, n, stream=stream)
 
     def sample(self, logits: torch.Tensor, temperature: float = 0.0, top_p: float = 1.0, seed: int = 0,
                counter: int = 0, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
