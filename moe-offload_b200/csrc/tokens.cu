@@ -278,7 +278,9 @@ static int launch_lm_head(const void *w, int V, int H, const void *x, int T, flo
     const int rows_per_block = (kHeadThreads / 32) * kHeadRowsPerWarp;
     const int grid = (V + rows_per_block - 1) / rows_per_block;
     auto kern = lm_head_kernel;
-    if (smem > 48u * 1024u)
+    // the kernel's own shared arrays count towards the 48 KB that need no opt-in (T * H = 12,288 sits
+    // on that border)
+    if (smem > 40u * 1024u)
         MOE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     kern<<<grid, kHeadThreads, smem, as_stream(stream)>>>(static_cast<const uint16_t *>(w), V, H,
                                                            static_cast<const uint16_t *>(x), T, logits, best);

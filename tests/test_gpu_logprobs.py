@@ -278,6 +278,15 @@ def test_head_against_definition(dev, T, V, H, n):
     check_head(w, x, None, n)
 
 
+def test_lm_head_rows_at_the_shared_memory_border(dev):
+    """T * H = 12,288: the staged rows alone are 48 KB, with the kernel's own arrays more."""
+    from moe_offload_b200.tokens import TokenHead
+    w, x, _ = head_case(dev, 6, 500, 2048, 21)
+    assert np.array_equal(TokenHead(w).logits(x[:4]).cpu().numpy(), exact_logits(w, x[:4]))
+    w, x, _ = head_case(dev, 4, 500, 3072, 22)
+    assert np.array_equal(TokenHead(w).logits(x).cpu().numpy(), exact_logits(w, x))
+
+
 def test_head_peaked_rows(dev):
     w, x, tg = head_case(dev, 40, 9000, 1024, 4, lean=30.0)
     r = check_head(w, x, tg, 6)
