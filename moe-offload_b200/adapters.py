@@ -92,7 +92,7 @@ class AdapterBank:
             if T:
                 call("moe_adapter_add", x.data_ptr(), T, self.K, self.N, self.a.data_ptr(), self.b.data_ptr(),
                      self.scale.data_ptr(), self.adapters, self.rank, ids.data_ptr(), y.data_ptr(),
-                     int(y.dtype == torch.float32), out.data_ptr(), _stream(stream))
+                     int(y.dtype == torch.float32), out.data_ptr(), _stream(stream, dev))
         return out
 
 

@@ -3,13 +3,17 @@
 //
 //   lse = log sum_v e^l_v      logprob = l_target - lse      entropy = lse - sum_v p_v l_v
 //
-// One pass over the row (4 V bytes: HBM, or L2 right after the LM head): every thread keeps the
-// softmax statistics of its elements (toplist.cuh) and its own largest element. The n largest
-// elements of a CTA's part all belong to the n threads with the largest maxima, so only those
-// threads' elements (V / threads each) are looked at a second time, instead of every element being
-// held against a running list. A row is shared by a cluster of up to 8 CTAs when there are few
-// rows; they join through distributed shared memory, so there is no workspace, no counter to
-// reset and one launch.
+// One pass over the row (4 V bytes: HBM, or L2 right after the LM head) by a cluster of up to 8
+// CTAs, one launch, no workspace. Every thread keeps the softmax statistics of its elements
+// (toplist.cuh) and, for the alternatives, the largest element of each of the 32 residues of the
+// index mod 32. The n-th largest of the row's 32 residue maxima is a bound tau that at least n
+// elements reach, and hardly more do (31 expected for n = 20 of independent logits), so only the
+// threads whose own maximum reaches tau look at their elements again (at one batch of 16, unless
+// another batch of theirs reaches tau too); the few that reach it are ranked by counting. No
+// running list, no sort.
+// Ties at tau (a mask that leaves fewer than n tokens, a row of equal logits) are taken in index
+// order from the start of the row; a row whose large elements crowd into fewer than n residues
+// takes n passes.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -23,6 +27,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kBatch = 4;              // chunks of 4 elements a thread has in flight
+constexpr int kCand = 256;             // elements above (or equal to) tau that are ranked at once
 
 struct LogprobArgs {
     const float *logits;
@@ -33,111 +39,274 @@ struct LogprobArgs {
     float *top_logprobs;
 };
 
-// 4 consecutive logits at virtual index 4 c - a (a: elements between the 16-byte boundary below
-// the row and the row), -inf outside the row; returns the index of v[0]
-MOE_D int load4(const float *row, int a, int V, int c, float (&v)[4]) {
-    const int i0 = 4 * c - a;
-    if (i0 >= 0 && i0 + 4 <= V) {
-        const float4 q = __ldg(reinterpret_cast<const float4 *>(row + i0));
-        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+// The row as chunks of 4 elements at 16-byte boundaries: chunk c holds the elements 4 c - a ..
+// 4 c - a + 3 (a: elements between the boundary below the row and the row), -inf outside the row.
+struct Row {
+    const float *p;
+    int a, V;
+    MOE_D float at(int i) const { return (i >= 0 && i < V) ? __ldg(p + i) : -INFINITY; }
+};
+
+// kBatch chunks c, c + kThreads, ...; lo, hi: the chunks that lie wholly inside the row and this
+// CTA's part; end: the part's end
+MOE_D void load_batch(const Row &row, int c, int lo, int hi, int end, float (&v)[4 * kBatch]) {
+    if (c >= lo && c + (kBatch - 1) * kThreads < hi) {
+        const float4 *q = reinterpret_cast<const float4 *>(row.p - row.a) + c;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const float4 f = __ldg(q + j * kThreads);
+            v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (i0 + i >= 0 && i0 + i < V) ? __ldg(row + i0 + i) : -INFINITY;
+        for (int j = 0; j < kBatch; ++j) {
+            const int cc = c + j * kThreads;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * j + i] = cc < end ? row.at(4 * cc - row.a + i) : -INFINITY;
+        }
     }
-    return i0;
+}
+
+// what a warp adds to the row's sums, relative to the row's largest value m: s, w as in Soft, and
+// how many threads hold m itself
+struct WarpSum {
+    float s, w;
+    int peaks;
+};
+
+struct Shared {
+    float res[kWarps][32];                       // residue maxima of the warps
+    float part_res[kMaxCluster][32];             // of the cluster's CTAs (written by them)
+    // gathered in the cluster's first CTA: every warp's sums and the candidates of the row
+    WarpSum sums[kMaxCluster * kWarps];
+    unsigned long long above[kCand], equal[kCand], out[kTopMax];
+    int nabove, nequal;
+    int scan[kWarps];
+    unsigned long long best[kWarps];
+};
+
+// appends the keys of the lanes with ok to a list of the first CTA, as far as it reaches
+MOE_D void append(unsigned long long *list, int *count, bool ok, unsigned long long key) {
+    const unsigned who = __ballot_sync(0xffffffffu, ok);
+    if (!who) return;
+    const int lane = threadIdx.x & 31;
+    int base = 0;
+    if (lane == __ffs(who) - 1) base = atomicAdd(count, __popc(who));
+    base = __shfl_sync(0xffffffffu, base, __ffs(who) - 1);
+    const int at = base + __popc(who & ((1u << lane) - 1u));
+    if (ok && at < kCand) list[at] = key;
+}
+
+// scatters the m keys of a list to out by their rank (+ from) among themselves, ranks below n
+MOE_D void rank_out(const unsigned long long *list, int m, int from, int n, unsigned long long *out) {
+    for (int i = threadIdx.x; i < m; i += kThreads) {
+        const unsigned long long k = list[i];
+        int r = from;
+        for (int j = 0; j < m; ++j) r += list[j] > k;
+        if (r < n) out[r] = k;
+    }
 }
 
 __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobArgs p) {
-    __shared__ unsigned long long lists[kWarps][32];
-    __shared__ Soft softs[kWarps];
-    __shared__ unsigned long long cta_list[32];
-    __shared__ Soft cta_soft;
+    __shared__ Shared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int t = blockIdx.x / parts;
-    const float *row = p.logits + (size_t)t * p.V;
-    const int a = (int)((reinterpret_cast<uintptr_t>(row) >> 2) & 3);
-    const int chunks = (p.V + a + 3) / 4;
+    const float *base = p.logits + (size_t)t * p.V;
+    const Row row{base, (int)((reinterpret_cast<uintptr_t>(base) >> 2) & 3), p.V};
+    const int chunks = (p.V + row.a + 3) / 4;
     const int per = (chunks + parts - 1) / parts;
     const int c0 = min(part * per, chunks), c1 = min(c0 + per, chunks);
+    const int lo = max(c0, row.a ? 1 : 0), hi = min(c1, (p.V + row.a) / 4);
+    if (tid == 0) sh.nabove = sh.nequal = 0;
+    if (parts > 1) cluster.barrier_arrive();     // waited for before the first store to another CTA
 
-    Soft st = soft_none();
-    // the first in-range index of the thread, for a thread whose elements are all -inf
-    int at = c0 + tid < c1 ? max(4 * (c0 + tid) - a, 0) : -1;
-#pragma unroll 4
-    for (int c = c0 + tid; c < c1; c += kThreads) {
-        float v[4];
-        const int i0 = load4(row, a, p.V, c, v);
-        soft_add(st, at, v, i0);
+    // ---- the pass over the row. best: the batch with the thread's first largest element, peak that
+    // element, next: the largest element of its other batches
+    SoftRun run = run_none();
+    float res[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    float next = -INFINITY;
+    int best = c0 + tid;
+#pragma unroll 1
+    for (int c = c0 + tid; c < c1; c += kThreads * kBatch) {
+        float v[4 * kBatch];
+        load_batch(row, c, lo, hi, c1, v);
+        float q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            q[i] = v[i];
+#pragma unroll
+            for (int j = 1; j < kBatch; ++j) q[i] = fmaxf(q[i], v[4 * j + i]);
+            res[i] = fmaxf(res[i], q[i]);
+        }
+        const float top = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
+        next = fmaxf(next, fminf(run.m, top));
+        if (top > run.m) best = c;
+        run_add(run, v, top);
     }
-    unsigned long long list = 0ull;
-    if (p.n > 0) {
-        // the CTA's 32 best thread maxima, sorted
-        list = top_sort(at >= 0 ? top_key(st.m, at) : 0ull);
-        lists[warp][lane] = list;
+    const float peak = run.m;
+    // lanes l, l + 8, l + 16, l + 24 hold the same residues 4 (l mod 8) .. + 3
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        res[i] = fmaxf(res[i], __shfl_xor_sync(0xffffffffu, res[i], 8));
+        res[i] = fmaxf(res[i], __shfl_xor_sync(0xffffffffu, res[i], 16));
     }
-    const Soft ws = soft_warp(st);
-    if (lane == 0) softs[warp] = ws;
+    if (lane < 8) *reinterpret_cast<float4 *>(&sh.res[warp][4 * lane]) = make_float4(res[0], res[1], res[2], res[3]);
     __syncthreads();
-    if (warp == 0) {
-        const Soft b = soft_warp(lane < kWarps ? softs[lane] : soft_none());
-        if (lane == 0) cta_soft = b;
+    // ---- the cluster's CTAs exchange their residue maxima
+    float top = sh.res[0][lane];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sh.res[w][lane]);
+    if (parts > 1) {
+        cluster.barrier_wait();
+        if (warp < parts) cluster.map_shared_rank(&sh.part_res[0][0], warp)[part * 32 + lane] = top;
+        cluster.sync();
+        top = sh.part_res[0][lane];
+        for (int q = 1; q < parts; ++q) top = fmaxf(top, sh.part_res[q][lane]);
     }
+    float m = top;                               // the row's largest value
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+
+    // ---- the sums relative to m; all its occurrences are left out and counted
+    {
+        const float d = fmaxf(run.r - m, kSoftFar), f = __expf(d);
+        const float e = fmaxf(peak - m, kSoftFar), g = peak == m ? 0.f : __expf(e);
+        WarpSum a{fmaf(f, run.s, g), fmaf(f, fmaf(d, run.s, run.w), e * g), peak == m};
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+            a.s += __shfl_xor_sync(0xffffffffu, a.s, off);
+            a.w += __shfl_xor_sync(0xffffffffu, a.w, off);
+            a.peaks += __shfl_xor_sync(0xffffffffu, a.peaks, off);
+        }
+        if (lane == 0) cluster.map_shared_rank(sh.sums, 0)[part * kWarps + warp] = a;
+    }
+    float tau = -INFINITY;
     if (p.n > 0) {
-        for (int h = kWarps / 2; h > 0; h >>= 1) {
-            if (warp < h) {
-                list = top_merge(list, lists[warp + h][lane]);
-                lists[warp][lane] = list;
-            }
-            __syncthreads();
+        int r = 0;                               // rank among the 32 residues, equal ones by lane
+#pragma unroll 4
+        for (int j = 0; j < 32; ++j) {
+            const float o = __shfl_sync(0xffffffffu, top, j);
+            r += (o > top || (o == top && j < lane)) ? 1 : 0;
         }
-        // every element that is among the CTA's n largest belongs to one of the first n of these
-        // threads and is not below the n-th of them
-        const unsigned long long floor_key = lists[0][p.n - 1];
-        list = 0ull;
-        for (int o = warp; o < p.n; o += kWarps) {
-            const unsigned long long ok = lists[0][o];
-            if (!ok) break;
-            const int oc = (top_index(ok) + a) >> 2;                 // a chunk of the owner
-            const int first = c0 + (oc - c0) % kThreads;             // its first one
-            for (int c = first; c < c1; c += kThreads * 8) {         // 8 chunks of 4 elements a pass
-                const int cc = c + kThreads * (lane >> 2), i = 4 * cc - a + (lane & 3);
-                unsigned long long k = 0ull;
-                if (cc < c1 && i >= 0 && i < p.V) k = top_key(__ldg(row + i), i);
-                list = top_insert(list, k, __ballot_sync(0xffffffffu, k >= floor_key && k != 0ull));
+        tau = __shfl_sync(0xffffffffu, top, __ffs(__ballot_sync(0xffffffffu, r == p.n - 1)) - 1);
+        // ---- the threads whose maximum reaches tau look again
+        unsigned long long *above = cluster.map_shared_rank(sh.above, 0), *equal = cluster.map_shared_rank(sh.equal, 0);
+        int *nabove = cluster.map_shared_rank(&sh.nabove, 0), *nequal = cluster.map_shared_rank(&sh.nequal, 0);
+        const bool mine = peak >= tau && peak > -INFINITY;
+        if (__ballot_sync(0xffffffffu, mine)) {
+            float v[4 * kBatch];
+            if (mine) load_batch(row, best, lo, hi, c1, v);
+#pragma unroll
+            for (int i = 0; i < 4 * kBatch; ++i) {
+                // (lanes that do not take part hold nothing: -inf is neither above tau nor equal to it)
+                const float x = mine ? v[i] : -INFINITY;
+                if (__ballot_sync(0xffffffffu, x >= tau && x > -INFINITY)) {
+                    const unsigned long long k = top_key(x, 4 * (best + (i >> 2) * kThreads) - row.a + (i & 3));
+                    append(above, nabove, x > tau, k);
+                    append(equal, nequal, x == tau && tau > -INFINITY, k);
+                }
+            }
+            // their other batches: the whole warp for one thread at a time, 128 elements a step
+            unsigned who = __ballot_sync(0xffffffffu, mine && next >= tau && next > -INFINITY);
+            while (who) {
+                const int owner = __ffs(who) - 1;
+                who &= who - 1;
+                const int ob = __shfl_sync(0xffffffffu, best, owner);
+                for (int c = c0 + 32 * warp + owner; c < c1; c += kThreads * 32) {
+                    float x[4];
+                    int at[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int cc = c + kThreads * (8 * j + (lane >> 2));
+                        const bool done = cc >= ob && cc < ob + kThreads * kBatch;       // the batch from above
+                        at[j] = 4 * cc - row.a + (lane & 3);
+                        x[j] = cc < c1 && !done ? row.at(at[j]) : -INFINITY;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        append(above, nabove, x[j] > tau, top_key(x[j], at[j]));
+                        append(equal, nequal, x[j] == tau && tau > -INFINITY, top_key(x[j], at[j]));
+                    }
+                }
             }
         }
-        __syncthreads();
-        lists[warp][lane] = list;
-        __syncthreads();
-        for (int h = kWarps / 2; h > 0; h >>= 1) {
-            if (warp < h) {
-                list = top_merge(list, lists[warp + h][lane]);
-                lists[warp][lane] = list;
-            }
-            __syncthreads();
-        }
-        if (warp == 0) cta_list[lane] = list;
     }
     if (parts > 1) cluster.sync();
-    if (part == 0 && warp == 0) {
-        __syncwarp();
-        Soft all = lane < parts ? *cluster.map_shared_rank(&cta_soft, lane) : soft_none();
-        all = soft_warp(all);
-        const float rest = soft_log_rest(all);
-        if (p.n > 0) {
-            unsigned long long other[kMaxCluster];
-#pragma unroll
-            for (int r = 1; r < kMaxCluster; ++r)
-                other[r] = r < parts ? cluster.map_shared_rank(cta_list, r)[lane] : 0ull;
-#pragma unroll
-            for (int r = 1; r < kMaxCluster; ++r)
-                if (r < parts) list = top_merge(list, other[r]);
-            if (lane < p.n) {
-                p.top_ids[(size_t)t * p.n + lane] = top_index(list);
-                p.top_logprobs[(size_t)t * p.n + lane] = (top_value(list) - all.m) - rest;
+    else __syncthreads();
+    if (part != 0) return;                       // only the first CTA's shared memory is used from here
+
+    const int n = p.n;
+    if (n > 0) {
+        const int na = sh.nabove, ne = sh.nequal;
+        if (na <= kCand) {
+            rank_out(sh.above, na, 0, n, sh.out);
+            if (tau > -INFINITY && ne <= kCand) {
+                rank_out(sh.equal, ne, na, n, sh.out);
+            } else {
+                // the first of the elements equal to tau, in index order (NaN counts as -inf)
+                const unsigned long long key0 = top_key(tau, 0) >> 32;
+                for (int i0 = 0, found = na; i0 < p.V && found < n; i0 += kThreads) {
+                    const int i = i0 + tid;
+                    const unsigned long long k = i < p.V ? top_key(__ldg(base + i), i) : 0ull;
+                    const bool ok = (k >> 32) == key0;
+                    const unsigned who = __ballot_sync(0xffffffffu, ok);
+                    if (lane == 0) sh.scan[warp] = __popc(who);
+                    __syncthreads();
+                    int before = found + __popc(who & ((1u << lane) - 1u));
+                    for (int w = 0; w < kWarps; ++w) {
+                        before += w < warp ? sh.scan[w] : 0;
+                        found += sh.scan[w];
+                    }
+                    if (ok && before < n) sh.out[before] = k;
+                    __syncthreads();
+                }
             }
+        } else {
+            // more than kCand elements above tau: the largest below the last one, n times
+            unsigned long long last = ~0ull;
+            for (int r = 0; r < n; ++r) {
+                unsigned long long b = 0ull;
+                for (int i = tid; i < p.V; i += kThreads) {
+                    const unsigned long long k = top_key(__ldg(base + i), i);
+                    if (k < last && k > b) b = k;
+                }
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) {
+                    const unsigned long long o = __shfl_xor_sync(0xffffffffu, b, off);
+                    b = o > b ? o : b;
+                }
+                if (lane == 0) sh.best[warp] = b;
+                __syncthreads();
+                for (int w = 0; w < kWarps; ++w) b = sh.best[w] > b ? sh.best[w] : b;
+                last = b;
+                if (tid == 0) sh.out[r] = b;
+                __syncthreads();
+            }
+        }
+        __syncthreads();
+    }
+    if (warp == 0) {
+        Soft all{m, 0.f, 0.f};
+        int peaks = 0;
+        for (int i = lane; i < parts * kWarps; i += 32) {
+            all.s += sh.sums[i].s;
+            all.w += sh.sums[i].w;
+            peaks += sh.sums[i].peaks;
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+            all.s += __shfl_xor_sync(0xffffffffu, all.s, off);
+            all.w += __shfl_xor_sync(0xffffffffu, all.w, off);
+            peaks += __shfl_xor_sync(0xffffffffu, peaks, off);
+        }
+        all.s += (float)(peaks - 1);             // Soft leaves one occurrence of m out
+        const float rest = soft_log_rest(all);
+        if (lane < n) {
+            const unsigned long long k = sh.out[lane];
+            p.top_ids[(size_t)t * n + lane] = top_index(k);
+            p.top_logprobs[(size_t)t * n + lane] = (top_value(k) - all.m) - rest;
         }
         if (lane == 0) {
             p.entropy[t] = soft_entropy(all);
@@ -145,11 +314,10 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobArgs p) {
                 const int id = p.targets[t];
                 const bool in = id >= 0 && id < p.V;
                 if (!in && id != -1) atomicOr(&g_moe_device_error, MOE_DEVERR_BAD_INPUT);
-                p.logprob[t] = in ? (__ldg(row + id) - all.m) - rest : __int_as_float(0x7fffffff);
+                p.logprob[t] = in ? (__ldg(base + id) - all.m) - rest : __int_as_float(0x7fffffff);
             }
         }
     }
-    if (parts > 1) cluster.sync();               // the others' shared memory stays until it is read
 }
 
 }  // namespace
@@ -157,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobArgs p) {
 int moe_token_logprobs_launch(const float *logits, int T, int V, const int32_t *targets, int n, float *logprob,
                               float *entropy, int32_t *top_ids, float *top_logprobs, void *stream) {
     int parts = 1;
-    while (parts < kMaxCluster && (long long)T * parts < 296 && V / (2 * parts) >= 4096) parts *= 2;
+    while (parts < kMaxCluster && (long long)T * parts < 148 && V / (2 * parts) >= 4096) parts *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)T * (unsigned)parts);
     cfg.blockDim = dim3(kThreads);

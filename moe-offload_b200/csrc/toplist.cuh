@@ -56,41 +56,45 @@ MOE_D Soft soft_warp(Soft a) {
     return a;
 }
 
-// Adds kN values (those with ok[i]) to a thread's statistics. at / idx: index of the thread's
-// first largest value; idx0 + i is the index of v[i]. NaN counts as -inf for the order.
+// The same statistics while a thread runs over its values: sums relative to a reference r that
+// stays within kRunSpan below the largest value m, so that most steps neither rescale nor branch.
+// The sums hold every value but the largest: a new value v adds min(m, v) and leaves max(m, v) out.
+struct SoftRun {
+    float m, r, s, w;
+};
+constexpr float kRunSpan = 32.f;       // e^32 * 2^30 values stay far inside fp32
+
+// the smaller of two, NaN if either is one
+MOE_D float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+MOE_D SoftRun run_none() { return SoftRun{-INFINITY, 0.f, 0.f, 0.f}; }
+
+// Adds kN values; top: the largest of them and of all before (NaN left out).
 template <int kN>
-MOE_D void soft_add(Soft &a, int &at, const float (&v)[kN], int idx0) {
-    float cm = v[0];
-#pragma unroll
-    for (int i = 1; i < kN; ++i) cm = fmaxf(cm, v[i]);
-    int skip = -1;
-    if (cm > a.m) {                              // the old largest becomes one of the others
-        if (a.m == -INFINITY) {
-            a.w = 0.f;
-        } else {
-            const float d = fmaxf(a.m - cm, kSoftFar), e = __expf(d);
-            a.w = e * (a.w + d * (a.s + 1.f));
-            a.s = (a.s + 1.f) * e;
-        }
-        a.m = cm;
-#pragma unroll
-        for (int i = kN - 1; i >= 0; --i)
-            if (v[i] == cm) skip = i;
-        at = idx0 + skip;
-    }
-    if (a.m == -INFINITY) {
-#pragma unroll
-        for (int i = 0; i < kN; ++i)
-            if (v[i] != v[i]) a.s = v[i];
-        return;
+MOE_D void run_add(SoftRun &a, const float (&v)[kN], float top) {
+    if (top > a.m && !(top <= a.r + kRunSpan && a.m > -INFINITY)) {
+        const float d = fmaxf(a.r - top, kSoftFar), f = a.m > -INFINITY ? __expf(d) : 1.f;
+        a.w = f * (a.w + d * a.s);
+        a.s *= f;                                // (nothing in the sums yet: 0, or NaN)
+        a.r = top;
     }
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-        const float d = v[i] - a.m;
-        const float e = i == skip ? 0.f : __expf(d);         // e^-inf = 0, NaN stays
+        const float d = min_nan(a.m, v[i]) - a.r, e = __expf(d);     // e^-inf = 0, NaN stays
+        a.m = fmaxf(a.m, v[i]);
         a.s += e;
-        a.w += fmaxf(d, kSoftFar) * e;
+        a.w = fmaf(fmaxf(d, kSoftFar), e, a.w);
     }
+}
+
+MOE_D Soft run_end(const SoftRun &a) {
+    if (a.m == -INFINITY) return Soft{a.m, a.s, 0.f};
+    const float d = fmaxf(a.r - a.m, kSoftFar), f = __expf(d);
+    return Soft{a.m, f * a.s, f * (a.w + d * a.s)};
 }
 
 // ------------------------------------------------------------------ order of the entries

@@ -23,9 +23,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream(stream) -> int:
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+def _stream(stream, dev: torch.device | None = None) -> int:
+    # (torch looks up the current device anew when it is not told which: several microseconds)
+    if stream is None:
+        stream = torch.cuda.current_stream() if dev is None else torch.cuda.current_stream(dev.index)
+    return stream.cuda_stream
 
 
 def _launch_on(dev: torch.device, stream):

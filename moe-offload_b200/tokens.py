@@ -60,7 +60,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, n:
         r = _logprob_outputs(T, V, targets, n, dev)
         if T:
             call("moe_token_logprobs", logits.data_ptr(), T, V, _ptr(targets), n, _ptr(r.logprob),
-                 r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), _stream(stream))
+                 r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), _stream(stream, dev))
     return r
 
 
@@ -81,7 +81,7 @@ def head_logprobs(head: torch.Tensor, h: torch.Tensor, targets: torch.Tensor | N
             ws = torch.empty(int(call("moe_head_logprobs_workspace_bytes", T, V, n)), dtype=torch.uint8, device=dev)
             call("moe_head_logprobs", head.data_ptr(), V, H, h.data_ptr(), T, _ptr(targets), n, _ptr(r.logprob),
                  r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), ws.data_ptr(), ws.numel(),
-                 _stream(stream))
+                 _stream(stream, dev))
     return r
 
 

@@ -105,6 +105,21 @@ def test_orders_and_ties(dev, V, order):
     check(np.stack([row, row[::-1], np.roll(row, 1)]).astype(np.float32), [0, V - 1, V // 2], n, dev)
 
 
+@pytest.mark.parametrize("V", [4096, 50021, 248320])
+def test_large_values_crowded(dev, V):
+    """Large elements that crowd into one residue, one thread's share or one end of the row."""
+    rng = np.random.default_rng(V)
+    lg = rng.normal(0, 1, (6, V)).astype(np.float32)
+    lg[0, ::32] += 50                                     # one residue mod 32, more than are ranked at once
+    lg[1, 5::2048] += 50
+    lg[2, :700] += 50
+    lg[3, -700:] += 50
+    lg[4, ::32] = 9.0                                     # ties there
+    lg[5, 3::64] = np.arange(lg[5, 3::64].size, dtype=np.float32)
+    for n in (1, 5, 20, 32):
+        check(lg, [0, 5, 6, V - 1, 32, 3], n, dev)
+
+
 def test_zero_signs_tie(dev):
     lg = np.array([[-0.0, 0.0, -0.0, 0.0, -1.0]], np.float32)
     check(lg, [1], 5, dev)
