@@ -32,10 +32,9 @@
 // token rows in shared memory) is one unit: the dequant warps wait for the tokens before they
 // arrive, so the MMA thread waits on one barrier per K-block and frees the stage with one
 // commit (two waits and two commits cost ~9 % more).
-#include <cuda.h>
-
 #include "common.cuh"
 #include "internal.h"
+#include "tcgen05.cuh"
 
 namespace {
 
@@ -43,21 +42,7 @@ constexpr int kBM = 128;          // weight rows per tile (MMA M)
 constexpr int kBK = 64;           // K per block (one 2-bit group)
 constexpr int kMaxBN = 128;       // tokens per tile (MMA N)
 
-// ------------------------------------------------------------------ tcgen05 / TMA helpers (PTX)
-
-// Shared-memory matrix descriptor for a K-major operand in the 128-byte-swizzle layout: rows
-// of 128 bytes (64 bf16 of K), 8-row groups 1024 bytes apart (stride byte offset), descriptor
-// version 1 (bits 46-47), layout type 2 = SWIZZLE_128B (bits 61-63). The K = 16 steps inside
-// a 64-wide block advance the start address by 32 bytes.
-MOE_D uint64_t desc_sw128(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-           (2ull << 61);
-}
-
-// instruction descriptor, kind::f16: D f32, A and B bf16, both K-major, N, M = 128
-MOE_HD uint32_t instr_desc_bf16(int n) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-}
+// ------------------------------------------------------------------ tcgen05 helpers (PTX)
 
 // A from tensor memory (lane = row, two bf16 of K per 32-bit column), B from shared memory
 MOE_D void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -65,11 +50,6 @@ MOE_D void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t id
         "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
         " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
         "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
-}
-
-MOE_D void mma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
 }
 
 MOE_D void tmem_ld16(uint32_t taddr, float (&v)[16]) {
@@ -97,51 +77,6 @@ MOE_D void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
 }
 
 MOE_D void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-MOE_D void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-MOE_D void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-MOE_D void mbar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
-// Bounded wait that also gives up once another warp of the CTA has aborted (the flag is
-// polled every 1024 tries). On its own timeout it records the device error and raises the
-// CTA's abort flag. Warp-uniform result: every lane of the calling warp must call it.
-MOE_D bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort) {
-    bool ok = false, gave_up = false;
-#pragma unroll 1
-    for (uint32_t i = 0; i < kMbarSpinLimit; ++i) {
-        if (mbar_try_wait(bar, parity)) {
-            ok = true;
-            break;
-        }
-        if ((i & 1023u) == 1023u && *abort) {
-            gave_up = true;
-            break;
-        }
-    }
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) {                                             // warp-uniform branch
-        const bool timed_out = !__any_sync(0xffffffffu, gave_up);
-        if ((threadIdx.x & 31) == 0) {
-            if (timed_out) atomicOr(&g_moe_device_error, MOE_DEVERR_MBAR_TIMEOUT);
-            *abort = 1;
-        }
-    }
-    return ok;
-}
-
-MOE_D bool aborted(volatile int *abort) { return __any_sync(0xffffffffu, *abort != 0); }
-
-// 2-D tiled TMA load (no multicast) completing on an mbarrier; x is the innermost coordinate
-MOE_D void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-            "r"(smem_addr(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
-        : "memory");
-}
 
 MOE_D uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     uint32_t d;
@@ -453,7 +388,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         for (int ti = blockIdx.x; ti < ntiles && !stop; ti += gridDim.x) {
             const Tile tl = a.tiles[ti];
             const int BN = (tl.n + 15) & ~15;
-            const uint32_t idesc = instr_desc_bf16(BN);
+            const uint32_t idesc = instr_desc_bf16(kBM, BN);
             const bool wide = BN > 64;
             const uint32_t h = nxt;
             if (aborted(abort)) break;
@@ -732,35 +667,6 @@ PrefillWs carve(void *base, int T, int H, int I, int E, int K) {
     return w;
 }
 
-// 2-D tensor map over a row-major [rows][cols] array with a box of box_cols x box_rows
-// elements and 128-byte swizzling (box_cols * element size = 128 bytes)
-int make_map(CUtensorMap *m, CUtensorMapDataType dt, size_t esize, const void *base, uint64_t cols, uint64_t rows,
-             uint32_t box_cols, uint32_t box_rows) {
-    const cuuint64_t dims[2] = {cols, rows};
-    const cuuint64_t strides[1] = {cols * esize};
-    const cuuint32_t box[2] = {box_cols, box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    // the driver entry point is looked up through the runtime, so the library does not link
-    // libcuda directly (it loads on hosts without a driver; calls then fail with an error)
-    using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static EncodeFn encode = nullptr;
-    if (!encode) {
-        void *fn = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        MOE_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
-        if (q != cudaDriverEntryPointSuccess || !fn)
-            return moe_set_error(MOE_ECUDA, "prefill: cuTensorMapEncodeTiled not available from the driver");
-        encode = reinterpret_cast<EncodeFn>(fn);
-    }
-    const CUresult r = encode(m, dt, 2, const_cast<void *>(base), dims, strides, box, estr,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return moe_set_error(MOE_ECUDA, "prefill: cuTensorMapEncodeTiled failed (%d)", (int)r);
-    return MOE_OK;
-}
-
 template <bool kGateUp, bool kFp16>
 int launch_gemm(const CUtensorMap &m0, const CUtensorMap &m1, const CUtensorMap &mb, const GemmArgs &g, int grid,
                 cudaStream_t st) {
@@ -842,13 +748,13 @@ int moe_prefill_experts_ex(const void *x, int T, int H, int I, int E, int K, con
     // tensor maps: codes [E*R rows][Kdim/16 words] (box 32 words x 128 rows = 8 K-blocks), the
     // expert-ordered x rows [T*K][H] and act [T*K][I] (16-row boxes)
     CUtensorMap mg, mu, mx, md, ma;
-    int rc = make_map(&mg, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, wg, (uint64_t)H / 16, (uint64_t)E * I, 32, kBM);
-    if (!rc) rc = make_map(&mu, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, wu, (uint64_t)H / 16, (uint64_t)E * I, 32, kBM);
+    int rc = make_map("prefill", &mg, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, wg, (uint64_t)H / 16, (uint64_t)E * I, 32, kBM);
+    if (!rc) rc = make_map("prefill", &mu, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, wu, (uint64_t)H / 16, (uint64_t)E * I, 32, kBM);
     // the gate/up B rows in expert order live in the yk buffer until the down GEMM overwrites it
     uint16_t *xs = w.yk;
-    if (!rc) rc = make_map(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, xs, (uint64_t)H, (uint64_t)TK, 64, 16);
-    if (!rc) rc = make_map(&md, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, wd, (uint64_t)I / 16, (uint64_t)E * H, 32, kBM);
-    if (!rc) rc = make_map(&ma, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, act, (uint64_t)I, (uint64_t)TK, 64, 16);
+    if (!rc) rc = make_map("prefill", &mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, xs, (uint64_t)H, (uint64_t)TK, 64, 16);
+    if (!rc) rc = make_map("prefill", &md, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, wd, (uint64_t)I / 16, (uint64_t)E * H, 32, kBM);
+    if (!rc) rc = make_map("prefill", &ma, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, act, (uint64_t)I, (uint64_t)TK, 64, 16);
     if (rc) return rc;
     if (reinterpret_cast<uintptr_t>(act) % 16) return moe_set_error(MOE_EINVAL, "prefill_experts: act_out not aligned");
     GemmArgs g1{w.tiles1, w.ntiles, H, I, K, static_cast<const uint16_t *>(sg), static_cast<const uint16_t *>(bg),
