@@ -1,16 +1,578 @@
 // Log-probabilities of given tokens, entropy and alternatives straight from hidden rows [T, H] and
-// the LM head [V, H] (prompt scoring): the values of moe_lm_head_logits followed by
-// moe_token_logprobs, four rows at a time through a [4, V] scratch.
+// the LM head [V, H] (prompt scoring), without [T, V] logits in memory.
+//
+//   score_kernel   the product X . W^T on the tensor cores (tcgen05, 128 rows x 256 vocabulary
+//                  entries a tile, fp32 accumulators in TMEM), each tile consumed where it lies: every
+//                  row keeps its running softmax statistics (toplist.cuh) and a list of its largest
+//                  logits. A CTA stays with one block of 128 rows and walks every P-th vocabulary
+//                  tile; CTAs of different row blocks walk the same tiles side by side, so the head
+//                  is read from HBM once and from L2 after that.
+//   finish_kernel  one CTA per row: joins the parts, sums the leading candidates' and the target's
+//                  logits again in 64 bits, exactly as the LM head does, corrects the statistics by
+//                  them and orders the alternatives.
+//   exact_kernel   rows whose order the candidates do not settle (more near-equal logits than a list
+//                  holds, values that are not finite): all V logits in 64 bits. It reads the rows'
+//                  number and ends when there are none.
+//
+// A tensor-core logit carries the rounding of H / 16 fp32 accumulations. That moves the log of the sum
+// of e^logit by the probability-weighted mean of those errors, a few 1e-7; it must not move an id or a
+// logit that is returned, hence the second sum. A candidate list is enough when the n-th exact logit
+// lies above the best logit outside by kMargin times the largest error seen among the row's
+// candidates, or when those errors are all zero.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "internal.h"
+#include "tcgen05.cuh"
+#include "toplist.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
-constexpr int kRows = 4;               // rows per pass of the LM head
+
+constexpr int kM = 128;                // rows of X per tile (MMA M)
+constexpr int kN = 256;                // vocabulary entries per tile (MMA N)
+constexpr int kK = 64;                 // K per stage: 128 bytes, the swizzle's width
+constexpr int kStages = 4;
+constexpr int kThreads = 320;          // TMA warp, MMA warp, 8 epilogue warps
+constexpr int kEpiWarps = 8;           // each 32 rows (its TMEM lanes) x half of the columns
+constexpr int kHalves = 2;
+constexpr uint32_t kABytes = kM * 128, kBBytes = kN * 128, kStageBytes = kABytes + kBBytes;
+constexpr uint32_t kTmemCols = 512;    // two accumulators of kN columns: one fills while one is read
+
+constexpr int kSlots = 64;             // a row's list in one part: kKeep kept, the rest to append to
+constexpr int kKeep = 40;              // n <= 32 and some to tell whether the order is settled
+constexpr int kMaxGroup = 16;          // row blocks per launch: 148 / 16 = 9 parts, 144 CTAs busy
+constexpr float kMargin = 16.f;
+
+struct ScoreArgs {
+    int T, V, H;                       // rows of this launch
+    int blocks, parts;                 // row blocks, vocabulary parts (grid = blocks * parts)
+    uint2 *lists;                      // [blocks * parts * kHalves][kSlots][kM] (value, index)
+    float4 *stats;                     // [blocks * parts * kHalves][kM] m, s, w, entries (as int bits)
+    int *redo;                         // [0]: rows for exact_kernel
+};
+
+struct ScoreSmem {
+    static constexpr size_t bars = (size_t)kStages * kStageBytes;
+    // full, empty [kStages]; acc_full, acc_empty [2]; drain; TMEM slot, abort flag
+    static constexpr size_t alloc = bars + (2 * kStages + 5) * 8 + 16 + 1024;
+};
+
+MOE_D void mma_bf16_ss(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
 
+// 32 columns of this warp's 32 TMEM lanes
+MOE_D void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// order-preserving image of a float that is no NaN (-0 below +0: both forms of a zero logit are
+// brought to +0 before); 0 is below all
+MOE_D uint32_t order_of(float f) {
+    const uint32_t u = __float_as_uint(f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// Cuts a thread's full list down to its kKeep largest entries, equal ones the lowest index first (the
+// entries are in index order, and stay so). Returns the smallest kept value. All 32 rows of the warp
+// work side by side: the kKeep-th largest is found bit by bit, by counting.
+MOE_D float list_cut(uint2 *list, int &count) {
+    uint32_t o[kSlots];
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) o[i] = i < count ? order_of(__uint_as_float(list[i * kM].x)) : 0u;
+    uint32_t bound = 0u;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = bound | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) n += o[i] >= c ? 1 : 0;
+        if (n >= kKeep) bound = c;
+    }
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) above += o[i] > bound ? 1 : 0;
+    int equal = kKeep - above, at = 0;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+        const bool tie = o[i] == bound && equal > 0;
+        if (o[i] > bound || tie) {
+            if (at != i) list[at * kM] = list[i * kM];
+            ++at;
+        }
+        equal -= tie ? 1 : 0;
+    }
+    count = at;
+    return __uint_as_float((bound & 0x80000000u) ? (bound & 0x7fffffffu) : ~bound);
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, ScoreArgs a) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + ScoreSmem::bars);
+    uint64_t *empty = full + kStages;
+    uint64_t *acc_full = empty + kStages;
+    uint64_t *acc_empty = acc_full + 2;
+    uint64_t *drain = acc_empty + 2;
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(drain + 1);
+    // set by the first failed wait of any role: the others stop, and what was issued is drained
+    volatile int *abort = reinterpret_cast<volatile int *>(tslot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], kEpiWarps);
+        }
+        mbar_init(drain, 1);
+        *abort = 0;
+        fence_barrier_init();
+        if (blockIdx.x == 0) *a.redo = 0;
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tslot)),
+                     "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tslot;
+    const int block = blockIdx.x % a.blocks, part = blockIdx.x / a.blocks;
+    const int tiles = (a.V + kN - 1) / kN, nkb = (a.H + kK - 1) / kK;
+
+    if (warp == 0) {
+        // ---- TMA: rows and columns outside the arrays arrive as zeros
+        uint32_t g = 0;
+        bool stop = false;
+        for (int v = part; v < tiles && !stop; v += a.parts) {
+            for (int kb = 0; kb < nkb; ++kb, ++g) {
+                const int s = g % kStages;
+                if (!wait_or_abort(&empty[s], ((g / kStages) & 1u) ^ 1u, abort)) {
+                    stop = true;
+                    break;
+                }
+                if (lane == 0) {
+                    unsigned char *st = smem + (size_t)s * kStageBytes;
+                    mbar_arrive_expect_tx(&full[s], kStageBytes);
+                    tma_load_2d(st, &map_x, kb * kK, block * kM, &full[s]);
+                    tma_load_2d(st + kABytes, &map_w, kb * kK, v * kN, &full[s]);
+                }
+                __syncwarp();
+            }
+        }
+        if (aborted(abort)) {
+            // no copy may still be writing shared memory when the CTA ends
+            for (uint32_t i = g > (uint32_t)kStages ? g - kStages : 0u; i < g; ++i)
+                mbar_wait(&full[i % kStages], (i / kStages) & 1u);
+        }
+    } else if (warp == 1) {
+        // ---- MMA: one thread issues
+        const uint32_t idesc = instr_desc_bf16(kM, kN);
+        uint32_t g = 0, it = 0;
+        bool stop = false, issued = false;
+        for (int v = part; v < tiles && !stop; v += a.parts, ++it) {
+            const uint32_t b = it & 1u;
+            if (aborted(abort) || !wait_or_abort(&acc_empty[b], ((it >> 1) & 1u) ^ 1u, abort)) break;
+            tc_fence_after();
+            for (int kb = 0; kb < nkb; ++kb, ++g) {
+                const int s = g % kStages;
+                if (!wait_or_abort(&full[s], (g / kStages) & 1u, abort)) {
+                    stop = true;
+                    break;
+                }
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint64_t da = desc_sw128(smem_addr(smem + (size_t)s * kStageBytes));
+                    const uint64_t db = desc_sw128(smem_addr(smem + (size_t)s * kStageBytes + kABytes));
+#pragma unroll
+                    for (int j = 0; j < kK / 16; ++j)
+                        mma_bf16_ss(tmem + b * kN, da + 2u * j, db + 2u * j, idesc, (kb | j) ? 1u : 0u);
+                    mma_commit(&empty[s]);
+                }
+                issued = true;
+                __syncwarp();
+            }
+            if (stop) break;
+            if (lane == 0) mma_commit(&acc_full[b]);
+            __syncwarp();
+        }
+        if (aborted(abort) && issued) {
+            if (lane == 0) mma_commit(drain);
+            __syncwarp();
+            mbar_wait(drain, 0);
+        }
+    } else {
+        // ---- epilogue: thread = row, 128 of the tile's columns
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const int lrow = quarter * 32 + lane, row = block * kM + lrow;
+        const int slice = (block * a.parts + part) * kHalves + half;
+        uint2 *list = a.lists + (size_t)slice * kSlots * kM + lrow;
+        const bool any = block * kM + quarter * 32 < a.T;           // a row of this warp is there
+        SoftRun run = run_none();
+        float least = row < a.T ? -INFINITY : INFINITY;              // appended: what is above it
+        int count = 0;
+        uint32_t it = 0;
+        for (int v = part; v < tiles; v += a.parts, ++it) {
+            const uint32_t b = it & 1u;
+            if (aborted(abort) || !wait_or_abort(&acc_full[b], (it >> 1) & 1u, abort)) break;
+            tc_fence_after();
+            const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + b * kN + half * (kN / 2);
+            const int col0 = v * kN + half * (kN / 2);
+            if (any) {
+#pragma unroll 1
+                for (int c = 0; c < kN / 2; c += 32) {
+                    float q[32];
+                    tmem_ld32(taddr + c, q);
+                    const int col = col0 + c;
+                    if (col + 32 > a.V) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (col + i >= a.V) q[i] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int h = 0; h < 32; h += 16) {
+                        float x[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] = q[h + i] + 0.f;
+                        float top = x[0];
+#pragma unroll
+                        for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+                        if (__any_sync(0xffffffffu, top > least)) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                if (x[i] > least) {
+                                    list[count * kM] = make_uint2(__float_as_uint(x[i]), (uint32_t)(col + h + i));
+                                    ++count;
+                                }
+                            }
+                            if (__any_sync(0xffffffffu, count > kSlots - 16)) {
+                                if (count > kKeep) least = list_cut(list, count);
+                                __syncwarp();
+                            }
+                        }
+                        run_add(run, x, top);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+        }
+        if (row < a.T) {
+            const Soft s = run_end(run);
+            a.stats[(size_t)slice * kM + lrow] = make_float4(s.m, s.s, s.w, __int_as_float(count));
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+}
+
+// ------------------------------------------------------------------ exact logits
+
+// x as floats, k-major (xs[k][c] = x[8 c + k]): lane-consecutive chunks read consecutive words
+MOE_D void stage_row(const uint16_t *x, int H, float *xs) {
+    const int nch = H / 8;
+    for (int i = threadIdx.x; i < H; i += blockDim.x) xs[(i & 7) * nch + (i >> 3)] = bf16_bits_to_f32(x[i]);
+}
+
+// A warp's dot product of a head row with the staged row: the products (exact in fp32) summed in
+// 64 bits in the LM head's order, rounded once
+MOE_D float exact_logit(const uint16_t *w, const float *xs, int H) {
+    const int lane = threadIdx.x & 31, nch = H / 8;
+    const uint4 *wr = reinterpret_cast<const uint4 *>(w);
+    double acc = 0.0;
+#pragma unroll 4
+    for (int c = lane; c < nch; c += 32) {
+        const uint4 q = __ldg(wr + c);
+        const uint32_t wv[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc += (double)(__uint_as_float(wv[j] << 16) * xs[(2 * j) * nch + c]);
+            acc += (double)(__uint_as_float(wv[j] & 0xffff0000u) * xs[(2 * j + 1) * nch + c]);
+        }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    return (float)acc;
+}
+
+// ------------------------------------------------------------------ one row's parts joined
+
+constexpr int kFinThreads = 512, kFinWarps = kFinThreads / 32;
+constexpr int kCand = 1024;            // candidates that are ranked at once
+
+struct FinishArgs {
+    const uint16_t *head, *x;          // x: this launch's first row
+    int V, H, n;
+    int blocks, parts;
+    const uint2 *lists;
+    const float4 *stats;
+    const int32_t *targets;
+    float *logprob, *entropy;
+    int32_t *top_ids;
+    float *top_logprobs;
+    int *redo;                         // [0] count, then (row, bits of m, bits of lse - m)
+};
+
+__global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
+    extern __shared__ float xs[];                                   // [H], k-major
+    __shared__ unsigned long long cand[kCand], lead[kKeep];
+    __shared__ float peaks[kFinThreads / 8], exact[kKeep + 1];
+    __shared__ Soft softs[kFinWarps];
+    __shared__ float tau_s;
+    __shared__ int ncand;
+    const int row = blockIdx.x, block = row / kM, lrow = row % kM;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int nlists = p.parts * kHalves;
+    const float4 *stats = p.stats + (size_t)block * nlists * kM + lrow;
+    const uint2 *lists = p.lists + (size_t)block * nlists * kSlots * kM + lrow;
+    stage_row(p.x + (size_t)row * p.H, p.H, xs);
+    if (tid == 0) {
+        ncand = 0;
+        tau_s = -INFINITY;
+    }
+
+    // statistics, in a fixed order
+    Soft st = soft_none();
+    for (int l = tid; l < nlists; l += kFinThreads) {
+        const float4 f = stats[(size_t)l * kM];
+        st = soft_merge(st, Soft{f.x, f.y, f.z});
+    }
+    st = soft_warp(st);
+    if (lane == 0) softs[warp] = st;
+
+    // the leading candidates: a bound from the maxima of 64 groups of threads, as in logprobs.cu
+    auto entries = [&](auto &&f) {
+        for (int l = warp; l < nlists; l += kFinWarps) {
+            const int count = min(max(__float_as_int(stats[(size_t)l * kM].w), 0), kSlots);
+            for (int i = lane; i < count; i += 32) f(lists[((size_t)l * kSlots + i) * kM]);
+        }
+    };
+    float top = -INFINITY;
+    entries([&](uint2 e) { top = fmaxf(top, __uint_as_float(e.x)); });
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if ((lane & 7) == 0) peaks[tid >> 3] = top;
+    __syncthreads();
+    if (tid < kFinThreads / 8) {
+        const float mine = peaks[tid];
+        int r = 0;
+        for (int j = 0; j < kFinThreads / 8; ++j) r += (peaks[j] > mine || (peaks[j] == mine && j < tid)) ? 1 : 0;
+        if (r == kKeep - 1) tau_s = mine;
+    }
+    st = soft_warp(lane < kFinWarps ? softs[lane] : soft_none());
+    __syncthreads();
+    const float tau = tau_s;
+    entries([&](uint2 e) {
+        if (__uint_as_float(e.x) >= tau) {
+            const int at = atomicAdd(&ncand, 1);
+            if (at < kCand) cand[at] = top_key(__uint_as_float(e.x), (int)e.y);
+        }
+    });
+    __syncthreads();
+    const int all = ncand, have = min(all, kCand);
+    for (int i = tid; i < have; i += kFinThreads) {
+        const unsigned long long k = cand[i];
+        int r = 0;
+        for (int j = 0; j < have; ++j) r += cand[j] > k ? 1 : 0;
+        if (r < kKeep) lead[r] = k;
+    }
+    __syncthreads();
+
+    // the leading ones' and the target's logits again, in 64 bits
+    const int lead_n = min(have, min(kKeep, max(p.n + 8, 8)));
+    const int target = p.targets ? p.targets[row] : -1;
+    const bool has_target = target >= 0 && target < p.V;
+    for (int i = warp; i <= lead_n; i += kFinWarps) {
+        const int id = i < lead_n ? top_index(lead[i]) : target;
+        const bool in = id >= 0 && id < p.V;
+        const float l = in ? exact_logit(p.head + (size_t)id * p.H, xs, p.H) : 0.f;
+        if (lane == 0) exact[i] = l;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+
+    // statistics relative to the exact logit of the leading candidate, which they leave out, with the
+    // others' exact logits in place of the tensor cores'
+    float err = 0.f;
+    Soft sum{0.f, 0.f, 0.f};
+    const bool fine = st.m < INFINITY && st.m > -INFINITY && st.s < INFINITY && lead_n > 0;
+    if (fine) {
+        sum.m = exact[0];
+        for (int i = lane; i < lead_n; i += 32) {
+            const float near = top_value(lead[i]), x = exact[i];
+            err = fmaxf(err, fabsf(x - near));
+            if (i > 0) {
+                const float dx = fmaxf(x - sum.m, kSoftFar), dn = fmaxf(near - sum.m, kSoftFar);
+                const float ex = __expf(dx), en = __expf(dn);
+                sum.s += ex - en;
+                sum.w += dx * ex - dn * en;
+            }
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+            sum.s += __shfl_xor_sync(0xffffffffu, sum.s, off);
+            sum.w += __shfl_xor_sync(0xffffffffu, sum.w, off);
+            err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, off));
+        }
+        const float d = st.m - sum.m, f = __expf(d);
+        sum.s = fmaxf(fmaf(f, st.s, sum.s), 0.f);
+        sum.w += f * (st.w + d * st.s);
+    } else {
+        sum.m = __int_as_float(0x7fffffff);
+    }
+    const float rest = soft_log_rest(sum);
+    if (lane == 0) {
+        p.entropy[row] = soft_entropy(sum);
+        if (p.targets) {
+            if (!has_target && target != -1) atomicOr(&g_moe_device_error, MOE_DEVERR_BAD_INPUT);
+            p.logprob[row] = has_target ? (exact[lead_n] - sum.m) - rest : __int_as_float(0x7fffffff);
+        }
+    }
+    if (p.n == 0) return;
+    // order by the exact logits (lead_n <= 64 entries: two a lane)
+    unsigned long long key[2], nth = 0ull;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = lane + 32 * h;
+        key[h] = i < lead_n ? top_key(exact[i], top_index(lead[i])) : 0ull;
+    }
+    int rank[2] = {0, 0};
+    for (int j = 0; j < lead_n; ++j) {
+        const unsigned long long o = __shfl_sync(0xffffffffu, key[j >> 5], j & 31);
+        rank[0] += o > key[0] ? 1 : 0;
+        rank[1] += o > key[1] ? 1 : 0;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const unsigned who = __ballot_sync(0xffffffffu, key[h] != 0ull && rank[h] == p.n - 1);
+        if (who) nth = __shfl_sync(0xffffffffu, key[h], __ffs(who) - 1);
+    }
+    // settled: there is nothing outside the candidates, or it cannot reach the n-th
+    const float outside = lead_n > 0 ? top_value(lead[lead_n - 1]) : INFINITY;
+    const bool settled = fine && all <= kCand && lead_n >= p.n &&
+                         (lead_n == p.V || (err == 0.f ? top_value(nth) >= outside
+                                                       : top_value(nth) > outside + kMargin * err));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (key[h] != 0ull && rank[h] < p.n) {
+            p.top_ids[(size_t)row * p.n + rank[h]] = top_index(key[h]);
+            p.top_logprobs[(size_t)row * p.n + rank[h]] = (top_value(key[h]) - sum.m) - rest;
+        }
+    }
+    if (!settled && lane == 0) {
+        const int at = atomicAdd(p.redo, 1);
+        p.redo[1 + 3 * at] = row;
+        p.redo[2 + 3 * at] = __float_as_int(sum.m);
+        p.redo[3 + 3 * at] = __float_as_int(rest);
+    }
+}
+
+// ------------------------------------------------------------------ rows the candidates do not settle
+
+constexpr int kExThreads = 512, kExWarps = kExThreads / 32, kExCluster = 8;
+
+struct ExactArgs {
+    const uint16_t *head, *x;
+    int V, H, n;
+    const int *redo;
+    int32_t *top_ids;
+    float *top_logprobs;
+};
+
+// a cluster of kExCluster CTAs per row: every warp keeps the best of its vocabulary entries
+__global__ void __cluster_dims__(kExCluster, 1, 1) __launch_bounds__(kExThreads) exact_kernel(ExactArgs p) {
+    extern __shared__ float xs[];
+    __shared__ unsigned long long lists[kExWarps][32], gathered[kExCluster][32];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rows = *p.redo, clusters = gridDim.x / kExCluster;
+    if (rows == 0) return;                                          // the same for every CTA
+    for (int i = blockIdx.x / kExCluster; i < rows; i += clusters) {
+        const int row = p.redo[1 + 3 * i];
+        stage_row(p.x + (size_t)row * p.H, p.H, xs);
+        __syncthreads();
+        unsigned long long list = 0ull;
+        for (int v = rank * kExWarps + warp; v < p.V; v += kExCluster * kExWarps) {
+            const unsigned long long k = top_key(exact_logit(p.head + (size_t)v * p.H, xs, p.H), v);
+            list = top_insert(list, k, 1u);
+        }
+        lists[warp][lane] = list;
+        __syncthreads();
+        for (int h = kExWarps / 2; h > 0; h >>= 1) {
+            if (warp < h) {
+                list = top_merge(list, lists[warp + h][lane]);
+                lists[warp][lane] = list;
+            }
+            __syncthreads();
+        }
+        cluster.sync();                                             // the first CTA has begun, and read the last row's
+        if (warp == 0) cluster.map_shared_rank(&gathered[0][0], 0)[rank * 32 + lane] = list;
+        cluster.sync();
+        if (rank == 0 && warp == 0) {
+            for (int r = 1; r < kExCluster; ++r) list = top_merge(list, gathered[r][lane]);
+            if (lane < p.n) {
+                const float m = __int_as_float(p.redo[2 + 3 * i]), rest = __int_as_float(p.redo[3 + 3 * i]);
+                p.top_ids[(size_t)row * p.n + lane] = top_index(list);
+                p.top_logprobs[(size_t)row * p.n + lane] = (top_value(list) - m) - rest;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+struct Plan {
+    int sms, blocks, parts;            // of the largest launch
+    size_t lists, stats, redo, bytes;  // offsets
+};
+
+int make_plan(int T, Plan &pl) {
+    int dev = 0;
+    MOE_CUDA_TRY(cudaGetDevice(&dev));
+    MOE_CUDA_TRY(cudaDeviceGetAttribute(&pl.sms, cudaDevAttrMultiProcessorCount, dev));
+    const int blocks = (T + kM - 1) / kM;
+    pl.blocks = blocks < kMaxGroup ? blocks : kMaxGroup;
+    pl.parts = pl.sms / pl.blocks;
+    const size_t slices = (size_t)pl.sms * kHalves;                // blocks * parts <= sms in every launch
+    pl.lists = 0;
+    pl.stats = al256(slices * kSlots * kM * sizeof(uint2));
+    pl.redo = pl.stats + al256(slices * kM * sizeof(float4));
+    pl.bytes = pl.redo + al256((1 + 3 * (size_t)pl.blocks * kM) * sizeof(int));
+    return MOE_OK;
+}
+
+}  // namespace
+
 extern "C" size_t moe_head_logprobs_workspace_bytes(int T, int V, int n) {
-    if (T <= 0 || V <= 0 || n < 0) return 0;
-    return (size_t)(T < kRows ? T : kRows) * V * sizeof(float);
+    Plan pl;
+    if (T <= 0 || V <= 0 || n < 0 || make_plan(T, pl) != MOE_OK) return 0;
+    return pl.bytes;
 }
 
 extern "C" int moe_head_logprobs(const void *head, int V, int H, const void *x, int T, const int32_t *targets, int n,
@@ -22,20 +584,44 @@ extern "C" int moe_head_logprobs(const void *head, int V, int H, const void *x, 
         return moe_set_error(MOE_EINVAL, "head logprobs: head and x must be set, H=%d a multiple of 8 up to 8192", H);
     if ((reinterpret_cast<uintptr_t>(head) | reinterpret_cast<uintptr_t>(x)) & 15)
         return moe_set_error(MOE_EINVAL, "head logprobs: head and x must be 16-byte aligned");
-    if (!workspace || workspace_bytes < moe_head_logprobs_workspace_bytes(T, V, n) ||
-        (reinterpret_cast<uintptr_t>(workspace) & 15))
-        return moe_set_error(MOE_EINVAL, "head logprobs: a 16-byte aligned workspace of %zu bytes is needed",
-                             moe_head_logprobs_workspace_bytes(T, V, n));
-    float *logits = static_cast<float *>(workspace);
-    const char *rows = static_cast<const char *>(x);
-    for (int t = 0; t < T; t += kRows) {
-        const int m = T - t < kRows ? T - t : kRows;
-        int rc = moe_lm_head_logits(head, V, H, rows + (size_t)t * H * 2, m, logits, stream);
-        if (rc != MOE_OK) return rc;
-        rc = moe_token_logprobs_launch(logits, m, V, targets ? targets + t : nullptr, n, logprob ? logprob + t : nullptr,
-                                       entropy + t, n ? top_ids + (size_t)t * n : nullptr,
-                                       n ? top_logprobs + (size_t)t * n : nullptr, stream);
-        if (rc != MOE_OK) return rc;
+    Plan pl;
+    if (int rc = make_plan(T, pl)) return rc;
+    if (!workspace || workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15))
+        return moe_set_error(MOE_EINVAL, "head logprobs: a 16-byte aligned workspace of %zu bytes is needed", pl.bytes);
+    char *ws = static_cast<char *>(workspace);
+    uint2 *lists = reinterpret_cast<uint2 *>(ws + pl.lists);
+    float4 *stats = reinterpret_cast<float4 *>(ws + pl.stats);
+    int *redo = reinterpret_cast<int *>(ws + pl.redo);
+    cudaStream_t st = as_stream(stream);
+    CUtensorMap mw, mx;
+    int rc = make_map("head logprobs", &mw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, head, (uint64_t)H, (uint64_t)V, kK, kN);
+    if (rc) return rc;
+    MOE_CUDA_TRY(cudaFuncSetAttribute(score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ScoreSmem::alloc));
+    const int tiles = (V + kN - 1) / kN;
+    for (int t0 = 0; t0 < T; t0 += kMaxGroup * kM) {
+        const int rows = T - t0 < kMaxGroup * kM ? T - t0 : kMaxGroup * kM;
+        const int blocks = (rows + kM - 1) / kM;
+        int parts = pl.sms / blocks;
+        if (parts > tiles) parts = tiles;
+        const uint16_t *xr = static_cast<const uint16_t *>(x) + (size_t)t0 * H;
+        if ((rc = make_map("head logprobs", &mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, xr, (uint64_t)H, (uint64_t)rows, kK,
+                           kM)))
+            return rc;
+        const ScoreArgs sa{rows, V, H, blocks, parts, lists, stats, redo};
+        score_kernel<<<blocks * parts, kThreads, ScoreSmem::alloc, st>>>(mx, mw, sa);
+        MOE_CUDA_TRY(cudaGetLastError());
+        int32_t *ids = n ? top_ids + (size_t)t0 * n : nullptr;
+        float *tl = n ? top_logprobs + (size_t)t0 * n : nullptr;
+        const FinishArgs fa{static_cast<const uint16_t *>(head), xr, V, H, n, blocks, parts, lists, stats,
+                            targets ? targets + t0 : nullptr, logprob ? logprob + t0 : nullptr, entropy + t0, ids, tl,
+                            redo};
+        finish_kernel<<<rows, kFinThreads, (size_t)H * sizeof(float), st>>>(fa);
+        MOE_CUDA_TRY(cudaGetLastError());
+        if (n > 0) {
+            const ExactArgs ea{static_cast<const uint16_t *>(head), xr, V, H, n, redo, ids, tl};
+            exact_kernel<<<(pl.sms / kExCluster) * kExCluster, kExThreads, (size_t)H * sizeof(float), st>>>(ea);
+            MOE_CUDA_TRY(cudaGetLastError());
+        }
     }
     return MOE_OK;
 }
