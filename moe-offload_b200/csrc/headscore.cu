@@ -40,14 +40,17 @@ constexpr int kHalves = 2;
 constexpr uint32_t kABytes = kM * 128, kBBytes = kN * 128, kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kTmemCols = 512;    // two accumulators of kN columns: one fills while one is read
 
-constexpr int kSlots = 64;             // a row's list in one part: kKeep kept, the rest to append to
-constexpr int kKeep = 40;              // n <= 32 and some to tell whether the order is settled
+constexpr int kSlots = 64;             // a row's list in one part: what is kept, and room to append to
+constexpr int kPad = 8;                // kept beyond n, to tell whether the order of the n is settled
+constexpr int kKeep = kTopMax + kPad;  // at most
+constexpr int kSpare = 4;
 constexpr int kMaxGroup = 16;          // row blocks per launch: 148 / 16 = 9 parts, 144 CTAs busy
 constexpr float kMargin = 16.f;
 
 struct ScoreArgs {
     int T, V, H;                       // rows of this launch
     int blocks, parts;                 // row blocks, vocabulary parts (grid = blocks * parts)
+    int keep;                          // entries a list has to keep
     uint2 *lists;                      // [blocks * parts * kHalves][kSlots][kM] (value, index)
     float4 *stats;                     // [blocks * parts * kHalves][kM] m, s, w, entries (as int bits)
     int *redo;                         // [0]: rows for exact_kernel
@@ -89,37 +92,62 @@ MOE_D uint32_t order_of(float f) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Cuts a thread's full list down to its kKeep largest entries, equal ones the lowest index first (the
-// entries are in index order, and stay so). Returns the smallest kept value. All 32 rows of the warp
-// work side by side: the kKeep-th largest is found bit by bit, by counting.
-MOE_D float list_cut(uint2 *list, int &count) {
+MOE_D float value_of(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
+
+// Cuts a thread's list (more than keep + kSpare entries) down to its keep largest entries, or up to
+// kSpare more where that ends the search sooner. Equal entries that do not all fit stay lowest index
+// first (the list is in index order, and stays so). Returns a value that at least keep of the kept
+// entries reach: what comes later and does not exceed it is not among the keep largest. The 32 rows of
+// a warp work side by side, each bisecting for its own bound by counting.
+MOE_D float list_cut(uint2 *list, int &count, int keep) {
     uint32_t o[kSlots];
+    uint32_t lo = 0xffffffffu, hi = 0u;
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) o[i] = i < count ? order_of(__uint_as_float(list[i * kM].x)) : 0u;
-    uint32_t bound = 0u;
-#pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = bound | (1u << bit);
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) n += o[i] >= c ? 1 : 0;
-        if (n >= kKeep) bound = c;
-    }
-    int above = 0;
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) above += o[i] > bound ? 1 : 0;
-    int equal = kKeep - above, at = 0;
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-        const bool tie = o[i] == bound && equal > 0;
-        if (o[i] > bound || tie) {
-            if (at != i) list[at * kM] = list[i * kM];
-            ++at;
+        hi = max(hi, o[i]);
+        lo = min(lo, o[i] ? o[i] : 0xffffffffu);
+    }
+    // at least keep entries reach lo, fewer reach hi
+    int reach = count;
+    hi += 1u;
+#pragma unroll 1
+    while (reach > keep + kSpare && hi - lo > 1u) {
+        const uint32_t mid = lo + (hi - lo) / 2u;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) n += o[i] >= mid ? 1 : 0;
+        if (n >= keep) {
+            lo = mid;
+            reach = n;
+        } else {
+            hi = mid;
         }
-        equal -= tie ? 1 : 0;
+    }
+    int ties = kSlots;                            // how many of those equal to lo stay
+    if (reach > keep + kSpare) {
+        ties = keep;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) ties -= o[i] > lo ? 1 : 0;
+    }
+    int at = 0;
+#pragma unroll
+    for (int i0 = 0; i0 < kSlots; i0 += 8) {      // 8 entries in flight (they are in L2)
+        uint2 e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (o[i0 + i] >= lo) e[i] = list[(i0 + i) * kM];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (o[i0 + i] > lo || (o[i0 + i] == lo && ties-- > 0)) {
+                list[at * kM] = e[i];
+                ++at;
+            }
+        }
     }
     count = at;
-    return __uint_as_float((bound & 0x80000000u) ? (bound & 0x7fffffffu) : ~bound);
+    return value_of(lo);
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -268,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 }
                             }
                             if (__any_sync(0xffffffffu, count > kSlots - 16)) {
-                                if (count > kKeep) least = list_cut(list, count);
+                                if (count > a.keep + kSpare) least = list_cut(list, count, a.keep);
                                 __syncwarp();
                             }
                         }
@@ -330,7 +358,7 @@ constexpr int kCand = 1024;            // candidates that are ranked at once
 struct FinishArgs {
     const uint16_t *head, *x;          // x: this launch's first row
     int V, H, n;
-    int blocks, parts;
+    int parts, keep;
     const uint2 *lists;
     const float4 *stats;
     const int32_t *targets;
@@ -343,7 +371,7 @@ struct FinishArgs {
 __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
     extern __shared__ float xs[];                                   // [H], k-major
     __shared__ unsigned long long cand[kCand], lead[kKeep];
-    __shared__ float peaks[kFinThreads / 8], exact[kKeep + 1];
+    __shared__ float peaks[kFinThreads], exact[kKeep + 1];
     __shared__ Soft softs[kFinWarps];
     __shared__ float tau_s;
     __shared__ int ncand;
@@ -367,29 +395,44 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
     st = soft_warp(st);
     if (lane == 0) softs[warp] = st;
 
-    // the leading candidates: a bound from the maxima of 64 groups of threads, as in logprobs.cu
-    auto entries = [&](auto &&f) {
+    // the leading candidates: the keep-th largest of many disjoint maxima is a bound that keep entries
+    // reach. With enough lists their own maxima do, and only the lists that reach the bound are read;
+    // else those of 64 groups of 8 threads
+    const bool by_list = nlists >= 2 * p.keep && nlists <= kFinThreads;
+    const int npeaks = by_list ? nlists : kFinThreads / 8;
+    auto entries = [&](float from, auto &&f) {
         for (int l = warp; l < nlists; l += kFinWarps) {
-            const int count = min(max(__float_as_int(stats[(size_t)l * kM].w), 0), kSlots);
-            for (int i = lane; i < count; i += 32) f(lists[((size_t)l * kSlots + i) * kM]);
+            const float4 s4 = stats[(size_t)l * kM];
+            if (s4.x < from) continue;
+            const int count = min(max(__float_as_int(s4.w), 0), kSlots);
+            const uint2 *e = lists + (size_t)l * kSlots * kM;
+            const bool a = lane < count, b = lane + 32 < count;
+            const uint2 ea = a ? e[lane * kM] : make_uint2(0u, 0u), eb = b ? e[(lane + 32) * kM] : make_uint2(0u, 0u);
+            if (a) f(ea);
+            if (b) f(eb);
         }
     };
-    float top = -INFINITY;
-    entries([&](uint2 e) { top = fmaxf(top, __uint_as_float(e.x)); });
+    if (by_list) {
+        if (tid < nlists) peaks[tid] = stats[(size_t)tid * kM].x;
+    } else {
+        float top = -INFINITY;
+        entries(-INFINITY, [&](uint2 e) { top = fmaxf(top, __uint_as_float(e.x)); });
 #pragma unroll
-    for (int off = 4; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    if ((lane & 7) == 0) peaks[tid >> 3] = top;
+        for (int off = 4; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if ((lane & 7) == 0) peaks[tid >> 3] = top;
+    }
     __syncthreads();
-    if (tid < kFinThreads / 8) {
+    if (tid < npeaks) {
         const float mine = peaks[tid];
         int r = 0;
-        for (int j = 0; j < kFinThreads / 8; ++j) r += (peaks[j] > mine || (peaks[j] == mine && j < tid)) ? 1 : 0;
-        if (r == kKeep - 1) tau_s = mine;
+#pragma unroll 8
+        for (int j = 0; j < npeaks; ++j) r += (peaks[j] > mine || (peaks[j] == mine && j < tid)) ? 1 : 0;
+        if (r == p.keep - 1) tau_s = mine;
     }
     st = soft_warp(lane < kFinWarps ? softs[lane] : soft_none());
     __syncthreads();
     const float tau = tau_s;
-    entries([&](uint2 e) {
+    entries(tau, [&](uint2 e) {
         if (__uint_as_float(e.x) >= tau) {
             const int at = atomicAdd(&ncand, 1);
             if (at < kCand) cand[at] = top_key(__uint_as_float(e.x), (int)e.y);
@@ -401,12 +444,12 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
         const unsigned long long k = cand[i];
         int r = 0;
         for (int j = 0; j < have; ++j) r += cand[j] > k ? 1 : 0;
-        if (r < kKeep) lead[r] = k;
+        if (r < p.keep) lead[r] = k;
     }
     __syncthreads();
 
     // the leading ones' and the target's logits again, in 64 bits
-    const int lead_n = min(have, min(kKeep, max(p.n + 8, 8)));
+    const int lead_n = min(have, p.keep);
     const int target = p.targets ? p.targets[row] : -1;
     const bool has_target = target >= 0 && target < p.V;
     for (int i = warp; i <= lead_n; i += kFinWarps) {
@@ -607,12 +650,12 @@ extern "C" int moe_head_logprobs(const void *head, int V, int H, const void *x, 
         if ((rc = make_map("head logprobs", &mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, xr, (uint64_t)H, (uint64_t)rows, kK,
                            kM)))
             return rc;
-        const ScoreArgs sa{rows, V, H, blocks, parts, lists, stats, redo};
+        const ScoreArgs sa{rows, V, H, blocks, parts, n + kPad, lists, stats, redo};
         score_kernel<<<blocks * parts, kThreads, ScoreSmem::alloc, st>>>(mx, mw, sa);
         MOE_CUDA_TRY(cudaGetLastError());
         int32_t *ids = n ? top_ids + (size_t)t0 * n : nullptr;
         float *tl = n ? top_logprobs + (size_t)t0 * n : nullptr;
-        const FinishArgs fa{static_cast<const uint16_t *>(head), xr, V, H, n, blocks, parts, lists, stats,
+        const FinishArgs fa{static_cast<const uint16_t *>(head), xr, V, H, n, parts, n + kPad, lists, stats,
                             targets ? targets + t0 : nullptr, logprob ? logprob + t0 : nullptr, entropy + t0, ids, tl,
                             redo};
         finish_kernel<<<rows, kFinThreads, (size_t)H * sizeof(float), st>>>(fa);
