@@ -7,8 +7,8 @@
 // a range of the N outputs. First u = x . A^T: the cluster's CTAs split K, their warps split it again,
 // and the partial sums (fp32) are added in a fixed order through distributed shared memory. Then each
 // CTA adds u . B^T to its share of the outputs. A tile goes through the adapters that its rows name, one
-// after another; rows of other adapters ride along in the products and are left out of the results,
-// so ids may come in any order.
+// after another; rows of other adapters ride along in the products and are left out of the results.
+// Ids may come in any order: where they come mixed, tiles gather the rows of one adapter.
 //
 // The products are 8 to 128 wide, far too little arithmetic per byte to be bound by the tensor cores
 // (rank 64: 60 FLOP per byte of x, y and out): mma.sync takes its operands from registers,
@@ -27,7 +27,8 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxRank = 128, kMaxCluster = 8;
-constexpr int kGroup = 32;             // outputs a warp takes at a time: 4 fragments of 8
+constexpr int kMaxSort = 1024;         // adapters up to which rows are gathered by adapter
+constexpr int kWindow = 4096;          // rows among which they are
 
 struct AdapterArgs {
     const uint16_t *x;
@@ -39,6 +40,8 @@ struct AdapterArgs {
     const void *y;
     void *out;
     int rows, splits;                  // rows per tile, ranges of N per tile
+    int sort;                          // gather rows by adapter where they come mixed
+    int vec;                           // rows of y and out start at 16-byte boundaries
 };
 
 MOE_D void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -49,7 +52,8 @@ MOE_D void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32
 }
 
 MOE_D uint32_t pack_bf16(float a, float b) {
-    return (uint32_t)f32_to_bf16_bits(a) | ((uint32_t)f32_to_bf16_bits(b) << 16);
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
 }
 
 // what a bf16 drops of v; nothing of what is not finite
@@ -63,62 +67,159 @@ template <int kMT, int kNT>
 struct Smem {
     static constexpr int kRows = 16 * kMT, kWK = kWarps / kMT;       // warps along K per row fragment
     static constexpr int kR = 8 * kNT, kSteps = (kR + 15) / 16;
+    static constexpr int kF = kNT == 2 ? 8 : 4;  // output fragments of 8 a warp takes at a time
     float part[kWK][kRows][kR];        // the warps' sums over their K steps
     float u[kRows][kR];                // the CTA's sums, read by the cluster
     uint4 frag[2][kMT][kSteps][32];    // scale * u as fragments: high and low parts
-    int id[kRows], kind[kRows];        // the rows' adapters; the different ones among them
-    unsigned long long member[kRows];  // which rows are of that kind
-    int kinds;
+    int row[kRows], id[kRows];         // the tile's rows and their adapters
+    int kind[kRows];                   // the different ones among them
+    unsigned member[kRows];            // which rows are of that kind
+    int kinds, sums[kWarps];
+    // gathering: the window's rows' adapters, and the places of each adapter's rows
+    uint16_t bin[kWindow];
+    int start[kMaxSort + 2], next[kMaxSort + 1];
 };
 
-template <bool kFp32, bool kVec>
-MOE_D void load8(const void *y, size_t at, int left, float (&v)[8]) {
-    if (kVec && left >= 8) {
+// 8 consecutive outputs as they lie in memory (left of them are inside the row)
+template <bool kFp32>
+struct Out8 {
+    uint32_t w[kFp32 ? 8 : 4];
+    MOE_D float get(int i) const {
+        return kFp32 ? __uint_as_float(w[i]) : __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    }
+    MOE_D void set2(int i, float a, float b) {       // outputs i (even) and i + 1
         if (kFp32) {
-            const float4 p = *reinterpret_cast<const float4 *>(static_cast<const float *>(y) + at);
-            const float4 q = *reinterpret_cast<const float4 *>(static_cast<const float *>(y) + at + 4);
-            v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
+            w[i] = __float_as_uint(a);
+            w[i + 1] = __float_as_uint(b);
         } else {
-            const uint4 p = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(y) + at);
-            const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+            w[i >> 1] = pack_bf16(a, b);
+        }
+    }
+    // whole: all 8 lie inside a row that starts at a 16-byte boundary
+    MOE_D void load(const void *y, size_t at, bool whole, int left) {
+        constexpr int kW = kFp32 ? 8 : 4;
+        if (whole) {
+            const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const char *>(y) + at * (kFp32 ? 4 : 2));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            for (int i = 0; i < kW / 4; ++i) {
+                const uint4 q = p[i];
+                w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+            }
+        } else if (kFp32) {
+#pragma unroll
+            for (int i = 0; i < kW; ++i) w[i] = i < left ? static_cast<const uint32_t *>(y)[at + i] : 0u;
+        } else {
+            const uint16_t *p = static_cast<const uint16_t *>(y) + at;
+#pragma unroll
+            for (int i = 0; i < kW; ++i)
+                w[i] = (2 * i < left ? (uint32_t)p[2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)p[2 * i + 1] << 16 : 0u);
+        }
+    }
+    MOE_D void store(void *out, size_t at, bool whole, int left) const {
+        constexpr int kW = kFp32 ? 8 : 4;
+        if (whole) {
+            uint4 *p = reinterpret_cast<uint4 *>(static_cast<char *>(out) + at * (kFp32 ? 4 : 2));
+#pragma unroll
+            for (int i = 0; i < kW / 4; ++i) p[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        } else if (kFp32) {
+#pragma unroll
+            for (int i = 0; i < kW; ++i)
+                if (i < left) static_cast<uint32_t *>(out)[at + i] = w[i];
+        } else {
+            uint16_t *p = static_cast<uint16_t *>(out) + at;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < left) p[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        }
+    }
+};
+
+// The rows of a tile, in sh.row / sh.id. Rows come in the order given when that keeps those of one
+// adapter together (a prompt's rows, one adapter for all); otherwise the rows of the tile's window are
+// taken in the order of their adapters (rows of one adapter in order, rows without one last): the tile
+// then holds few adapters, and each is read by few tiles.
+template <class S>
+MOE_D int tile_rows(S &sh, const AdapterArgs &p, int tile, bool report) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = kWindow / p.rows, w0 = tile / per * per * p.rows, wn = min(p.T - w0, per * p.rows);
+    const int at = tile * p.rows - w0, rows = min(p.rows, wn - at);
+    const int32_t *ids = p.ids + w0;
+    bool mixed = false;
+    if (p.sort) {
+        int runs = 0;
+        for (int t = tid; t < wn; t += kThreads) {
+            const int id = ids[t];
+            runs += t == 0 || id != ids[t - 1] ? 1 : 0;
+            const bool in = id >= 0 && id < p.adapters;
+            if (!in && id != -1 && report) atomicOr(&g_moe_device_error, MOE_DEVERR_BAD_INPUT);
+            sh.bin[t] = (uint16_t)(in ? id : p.adapters);
+        }
+        for (int i = tid; i <= p.adapters; i += kThreads) sh.next[i] = 0;
+        runs = __reduce_add_sync(0xffffffffu, runs);
+        if (lane == 0) sh.sums[warp] = runs;
+        __syncthreads();
+        runs = 0;
+        for (int w = 0; w < kWarps; ++w) runs += sh.sums[w];
+        mixed = runs * p.rows > 2 * wn;          // runs shorter than half a tile
+    }
+    if (tid < S::kRows) {
+        int id = -1;
+        if (tid < rows) {
+            id = p.sort ? (int)sh.bin[at + tid] : ids[at + tid];
+            if (p.sort && id == p.adapters) id = -1;
+            if (id < -1 || id >= p.adapters) {
+                if (report) atomicOr(&g_moe_device_error, MOE_DEVERR_BAD_INPUT);
+                id = -1;
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = i >= left ? 0.f : kFp32 ? static_cast<const float *>(y)[at + i]
-                                           : bf16_bits_to_f32(static_cast<const uint16_t *>(y)[at + i]);
+        sh.row[tid] = w0 + at + min(tid, rows - 1);
+        sh.id[tid] = id;
     }
+    if (!mixed) {
+        __syncthreads();
+        return rows;
+    }
+    for (int t = tid; t < wn; t += kThreads) atomicAdd(&sh.next[sh.bin[t]], 1);
+    __syncthreads();
+    if (warp == 0) {
+        int before = 0;                          // places: an exclusive scan of the counts
+        for (int i0 = 0; i0 <= p.adapters; i0 += 32) {
+            const int i = i0 + lane, c = i <= p.adapters ? sh.next[i] : 0;
+            int sum = c;
+            for (int off = 1; off < 32; off <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, sum, off);
+                if (lane >= off) sum += o;
+            }
+            if (i <= p.adapters) sh.start[i] = sh.next[i] = before + sum - c;
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) sh.start[p.adapters + 1] = before;
+        __syncwarp();
+        for (int t0 = 0; t0 < wn; t0 += 32) {    // in row order, for the adapters that reach the tile
+            const int t = t0 + lane, b = t < wn ? sh.bin[t] : -1;
+            unsigned todo = __ballot_sync(0xffffffffu, b >= 0 && sh.start[b] < at + rows && sh.start[b + 1] > at);
+            while (todo) {
+                const int k = __shfl_sync(0xffffffffu, b, __ffs(todo) - 1);
+                const unsigned who = __ballot_sync(0xffffffffu, b == k);
+                todo &= ~who;
+                const int first = sh.next[k] - at, place = first + __popc(who & ((1u << lane) - 1u));
+                if (b == k && place >= 0 && place < rows) {
+                    sh.row[place] = w0 + t;
+                    sh.id[place] = b < p.adapters ? b : -1;
+                }
+                __syncwarp();
+                if (lane == 0) sh.next[k] = first + at + __popc(who);
+                __syncwarp();
+            }
+        }
+    }
+    __syncthreads();
+    return rows;
 }
 
-template <bool kFp32, bool kVec>
-MOE_D void store8(void *out, size_t at, int left, const float (&v)[8]) {
-    if (kVec && left >= 8) {
-        if (kFp32) {
-            float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
-            o[0] = make_float4(v[0], v[1], v[2], v[3]);
-            o[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + at) = make_uint4(
-                pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (i >= left) break;
-            if (kFp32) static_cast<float *>(out)[at + i] = v[i];
-            else static_cast<uint16_t *>(out)[at + i] = f32_to_bf16_bits(v[i]);
-        }
-    }
-}
-
-// kVec: rows of y and out start at 16-byte boundaries
-template <int kMT, int kNT, bool kFp32, bool kVec>
-__global__ void __launch_bounds__(kThreads) adapter_kernel(AdapterArgs p) {
+// two CTAs an SM where the registers allow it: the kernel is a chain of short dependent phases
+template <int kMT, int kNT, bool kFp32>
+__global__ void __launch_bounds__(kThreads, kNT <= 8 ? 2 : 1) adapter_kernel(AdapterArgs p) {
     using S = Smem<kMT, kNT>;
     extern __shared__ __align__(16) unsigned char smem[];
     S &sh = *reinterpret_cast<S *>(smem);
@@ -126,35 +227,21 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(AdapterArgs p) {
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
     const int unit = blockIdx.x / ctas, tile = unit / p.splits, split = unit % p.splits;
-    const int t0 = tile * p.rows, rows = min(p.rows, p.T - t0);
+    const int rows = tile_rows(sh, p, tile, rank == 0 && split == 0);
 
     // ---- the adapters of the tile, in the order of their first rows
-    if (tid < S::kRows) {
-        int id = tid < rows ? p.ids[t0 + tid] : -1;
-        if (id < -1 || id >= p.adapters) {
-            if (rank == 0 && split == 0) atomicOr(&g_moe_device_error, MOE_DEVERR_BAD_INPUT);
-            id = -1;
-        }
-        sh.id[tid] = id;
-    }
-    __syncthreads();
     if (warp == 0) {
-        int n = 0;
-#pragma unroll
-        for (int h = 0; h < S::kRows; h += 32) {
-            const int r = h + lane;
-            const int id = r < S::kRows ? sh.id[r] : -1;
-            unsigned long long same = 0ull;
-#pragma unroll 1
-            for (int j = 0; j < S::kRows; ++j) same |= (unsigned long long)(sh.id[j] == id) << j;
-            const bool first = id >= 0 && __ffsll((long long)same) - 1 == r;
-            const unsigned who = __ballot_sync(0xffffffffu, first);
-            if (first) {
-                const int at = n + __popc(who & ((1u << lane) - 1u));
-                sh.kind[at] = id;
-                sh.member[at] = same;
+        int id = lane < S::kRows ? sh.id[lane] : -1, n = 0;
+        unsigned todo = __ballot_sync(0xffffffffu, id >= 0);
+        while (todo) {
+            const int k = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
+            const unsigned who = __ballot_sync(0xffffffffu, id == k);
+            todo &= ~who;
+            if (lane == 0) {
+                sh.kind[n] = k;
+                sh.member[n] = who;
             }
-            n += __popc(who);
+            ++n;
         }
         if (lane == 0) sh.kinds = n;
     }
@@ -168,27 +255,29 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(AdapterArgs p) {
         const int steps = (p.K + 31) / 32, per = (steps + ctas - 1) / ctas;
         const int s1 = min((rank + 1) * per, steps);
         const int ra = 16 * mt + g, rb = ra + 8;
-        const uint16_t *xa = p.x + (size_t)(t0 + ra) * p.K + 8 * q, *xb = p.x + (size_t)(t0 + rb) * p.K + 8 * q;
+        const uint16_t *xa = p.x + (size_t)sh.row[ra] * p.K + 8 * q, *xb = p.x + (size_t)sh.row[rb] * p.K + 8 * q;
         const bool oka = ra < rows, okb = rb < rows;
         for (int d = 0; d < kinds; ++d) {
-            if (!((sh.member[d] >> (16 * mt)) & 0xffffull)) continue;             // none of this warp's rows
+            if (!((sh.member[d] >> (16 * mt)) & 0xffffu)) continue;               // none of this warp's rows
             const uint16_t *ar = p.a + ((size_t)sh.kind[d] * p.rank + g) * p.K + 8 * q;
             float acc[kNT][4] = {};
-#pragma unroll 2
+#pragma unroll (kNT <= 4 ? 4 : kNT <= 8 ? 2 : 1)
             for (int s = rank * per + wk; s < s1; s += S::kWK) {
                 const bool in = 32 * s + 8 * q < p.K;
                 const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-                const uint4 va = in && oka ? *reinterpret_cast<const uint4 *>(xa + 32 * s) : zero;
-                const uint4 vb = in && okb ? *reinterpret_cast<const uint4 *>(xb + 32 * s) : zero;
+                const uint4 va = in && oka ? __ldg(reinterpret_cast<const uint4 *>(xa + 32 * s)) : zero;
+                const uint4 vb = in && okb ? __ldg(reinterpret_cast<const uint4 *>(xb + 32 * s)) : zero;
+                const uint16_t *as = ar + 32 * s;
                 uint4 w[kNT];
 #pragma unroll
-                for (int j = 0; j < kNT; ++j)
-                    w[j] = in && j < nt ? __ldg(reinterpret_cast<const uint4 *>(ar + (size_t)8 * j * p.K + 32 * s)) : zero;
-#pragma unroll
                 for (int j = 0; j < kNT; ++j) {
-                    mma16816(acc[j], va.x, vb.x, va.y, vb.y, w[j].x, w[j].y);
-                    mma16816(acc[j], va.z, vb.z, va.w, vb.w, w[j].z, w[j].w);
+                    w[j] = in && j < nt ? __ldg(reinterpret_cast<const uint4 *>(as)) : zero;
+                    as += 8 * p.K;
                 }
+#pragma unroll
+                for (int j = 0; j < kNT; ++j) mma16816(acc[j], va.x, vb.x, va.y, vb.y, w[j].x, w[j].y);
+#pragma unroll
+                for (int j = 0; j < kNT; ++j) mma16816(acc[j], va.z, vb.z, va.w, vb.w, w[j].z, w[j].w);
             }
             const bool mine = sh.id[ra] == sh.kind[d], mineb = sh.id[rb] == sh.kind[d];
 #pragma unroll
@@ -235,72 +324,101 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(AdapterArgs p) {
         sh.frag[0][m][s][l] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         sh.frag[1][m][s][l] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
-    if (ctas > 1) cluster.sync();                // (the others have read this CTA's u)
-    else __syncthreads();
+    __syncthreads();
+    if (ctas > 1) cluster.barrier_arrive();      // this CTA has read the others' u (waited for at the end)
 
-    // ---- out = y + u . B^T, 32 outputs a warp at a time: fragment f, place (q, e) is output
-    // n0 + 8 q + 2 f + e, so that a lane ends with 8 consecutive ones
-    const int groups = (p.N + kGroup - 1) / kGroup, shares = p.splits * ctas;
+    // ---- out = y + u . B^T, kCols outputs a warp at a time: fragment f, place (q, e) is output
+    // n0 + 32 (f / 4) + 8 q + 2 (f % 4) + e, so that a lane ends with runs of 8 consecutive ones
+    constexpr int kF = S::kF, kCols = 8 * kF, kChunk = S::kSteps < 4 ? S::kSteps : 4;
+    const int groups = (p.N + kCols - 1) / kCols, shares = p.splits * ctas;
     const int share = split * ctas + rank;
-    const int gper = (groups + shares - 1) / shares, g1 = min((share + 1) * gper, groups);
+    const int gper = (groups + shares - 1) / shares, g0 = min(share * gper, groups), g1 = min(g0 + gper, groups);
     const int steps = (p.rank + 15) / 16;
-    for (int gr = share * gper + warp; gr < g1; gr += kWarps) {
-        const int n0 = gr * kGroup, left = p.N - (n0 + 8 * q);
-        float acc[kMT][4][4] = {};
+    size_t at[kMT][2];                           // the lane's rows in y and out
+#pragma unroll
+    for (int m = 0; m < kMT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) at[m][h] = (size_t)sh.row[16 * m + g + 8 * h] * p.N + 8 * q;
+    for (int gr = g0 + warp; gr < g1; gr += kWarps) {
+        const int n0 = gr * kCols, left = p.N - n0 - 8 * q;
+        const bool inner = n0 + kCols <= p.N, whole = inner && p.vec;              // (warp-uniform)
+        // fragment column g of fragment f: output n0 + 32 (f / 4) + 8 (g / 2) + 2 (f % 4) + g % 2
+        const int nb = n0 + 8 * (g >> 1) + (g & 1);
         for (int d = 0; d < kinds; ++d) {
-            const unsigned long long member = sh.member[d];
-            // fragment column g of fragment f: output n0 + 8 (g / 2) + 2 f + g % 2
-            const int nb = n0 + 8 * (g >> 1) + (g & 1);
+            const unsigned member = sh.member[d] >> g;
+            Out8<kFp32> v[kMT][2][kF / 4];
+#pragma unroll
+            for (int m = 0; m < kMT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int c = 0; c < kF / 4; ++c)
+                        if (member & (1u << (16 * m + 8 * h)))
+                            v[m][h][c].load(p.y, at[m][h] + n0 + 32 * c, whole, left - 32 * c);
+            float sum[kMT][kF][4] = {};
             const uint16_t *br = p.b + ((size_t)sh.kind[d] * p.N + nb) * p.rank + 4 * q;
-            float sum[kMT][4][4] = {};
-#pragma unroll 2
-            for (int s = 0; s < steps; ++s) {
-                uint2 w[4];
 #pragma unroll
-                for (int f = 0; f < 4; ++f)
-                    w[f] = nb + 2 * f < p.N && 16 * s + 4 * q < p.rank
-                               ? __ldg(reinterpret_cast<const uint2 *>(br + (size_t)2 * f * p.rank + 16 * s))
-                               : make_uint2(0u, 0u);
+            for (int s0 = 0; s0 < S::kSteps; s0 += kChunk) {
+                if (s0 >= steps) break;
+                uint2 w[kChunk][kF];
 #pragma unroll
-                for (int m = 0; m < kMT; ++m) {
-                    if (kMT > 1 && !((member >> (16 * m)) & 0xffffull)) continue;
-                    const uint4 hi = sh.frag[0][m][s][lane], lo = sh.frag[1][m][s][lane];
+                for (int f = 0; f < kF; ++f) {
+                    const int n = 32 * (f >> 2) + 2 * (f & 3);
+                    const uint16_t *bf = br + n * p.rank + 16 * s0;
+                    const bool in = inner || nb + n < p.N;
 #pragma unroll
-                    for (int f = 0; f < 4; ++f) {
-                        mma16816(sum[m][f], hi.x, hi.y, hi.z, hi.w, w[f].x, w[f].y);
-                        mma16816(sum[m][f], lo.x, lo.y, lo.z, lo.w, w[f].x, w[f].y);
+                    for (int s = 0; s < kChunk; ++s)
+                        w[s][f] = in && 16 * (s0 + s) + 4 * q < p.rank ? __ldg(reinterpret_cast<const uint2 *>(bf + 16 * s))
+                                                                       : make_uint2(0u, 0u);
+                }
+#pragma unroll
+                for (int s = 0; s < kChunk; ++s) {
+                    if (s0 + s >= steps) break;
+#pragma unroll
+                    for (int m = 0; m < kMT; ++m) {
+                        if (kMT > 1 && !(sh.member[d] & (0xffffu << (16 * m)))) continue;
+                        const uint4 hi = sh.frag[0][m][s0 + s][lane], lo = sh.frag[1][m][s0 + s][lane];
+#pragma unroll
+                        for (int f = 0; f < kF; ++f) mma16816(sum[m][f], hi.x, hi.y, hi.z, hi.w, w[s][f].x, w[s][f].y);
+#pragma unroll
+                        for (int f = 0; f < kF; ++f) mma16816(sum[m][f], lo.x, lo.y, lo.z, lo.w, w[s][f].x, w[s][f].y);
                     }
                 }
             }
 #pragma unroll
-            for (int m = 0; m < kMT; ++m) {
-                const bool ma = (member >> (16 * m + g)) & 1ull, mb = (member >> (16 * m + g + 8)) & 1ull;
+            for (int m = 0; m < kMT; ++m)
 #pragma unroll
-                for (int f = 0; f < 4; ++f) {
-                    if (ma) { acc[m][f][0] = sum[m][f][0]; acc[m][f][1] = sum[m][f][1]; }
-                    if (mb) { acc[m][f][2] = sum[m][f][2]; acc[m][f][3] = sum[m][f][3]; }
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int c = 0; c < kF / 4; ++c) {
+                        if (!(member & (1u << (16 * m + 8 * h)))) continue;
+                        Out8<kFp32> &o = v[m][h][c];
+#pragma unroll
+                        for (int f = 0; f < 4; ++f)
+                            o.set2(2 * f, o.get(2 * f) + sum[m][4 * c + f][2 * h],
+                                   o.get(2 * f + 1) + sum[m][4 * c + f][2 * h + 1]);
+                        o.store(p.out, at[m][h] + n0 + 32 * c, whole, left - 32 * c);
+                    }
+        }
+    }
+    if (p.out != p.y) {                          // rows without an adapter keep their bits
+#pragma unroll
+        for (int i = 0; i < 2 * kMT; ++i) {
+            const int r = 8 * i + g;
+            if (r >= rows || sh.id[r] >= 0) continue;
+            for (int gr = g0 + warp; gr < g1; gr += kWarps) {
+                const int n0 = gr * kCols, left = p.N - n0 - 8 * q;
+                const bool whole = n0 + kCols <= p.N && p.vec;
+#pragma unroll
+                for (int c = 0; c < kF / 4; ++c) {
+                    Out8<kFp32> v;
+                    v.load(p.y, at[i / 2][i % 2] + n0 + 32 * c, whole, left - 32 * c);
+                    v.store(p.out, at[i / 2][i % 2] + n0 + 32 * c, whole, left - 32 * c);
                 }
             }
         }
-#pragma unroll
-        for (int m = 0; m < kMT; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = 16 * m + g + 8 * h;
-                if (r >= rows || left <= 0) continue;
-                const size_t at = (size_t)(t0 + r) * p.N + n0 + 8 * q;
-                float v[8];
-                load8<kFp32, kVec>(p.y, at, left, v);
-                if (sh.id[r] >= 0) {                                // (a kept row keeps its bits, NaN too)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) {
-                        v[2 * f] += acc[m][f][2 * h];
-                        v[2 * f + 1] += acc[m][f][2 * h + 1];
-                    }
-                }
-                store8<kFp32, kVec>(p.out, at, left, v);
-            }
     }
+    if (ctas > 1) cluster.barrier_wait();        // its own u stays until the others have read it
 }
 
 bool overlap(const void *a, size_t na, const void *b, size_t nb) {
@@ -308,9 +426,9 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb) {
     return p < q + nb && q < p + na;
 }
 
-template <int kMT, int kNT, bool kFp32, bool kVec>
+template <int kMT, int kNT, bool kFp32>
 int launch(const AdapterArgs &p, int ctas, cudaStream_t st) {
-    auto kern = adapter_kernel<kMT, kNT, kFp32, kVec>;
+    auto kern = adapter_kernel<kMT, kNT, kFp32>;
     const size_t smem = sizeof(Smem<kMT, kNT>);
     MOE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
@@ -329,17 +447,16 @@ int launch(const AdapterArgs &p, int ctas, cudaStream_t st) {
 }
 
 template <int kMT, int kNT>
-int dispatch_y(const AdapterArgs &p, int ctas, bool fp32, bool vec, cudaStream_t st) {
-    if (fp32) return vec ? launch<kMT, kNT, true, true>(p, ctas, st) : launch<kMT, kNT, true, false>(p, ctas, st);
-    return vec ? launch<kMT, kNT, false, true>(p, ctas, st) : launch<kMT, kNT, false, false>(p, ctas, st);
+int dispatch_y(const AdapterArgs &p, int ctas, bool fp32, cudaStream_t st) {
+    return fp32 ? launch<kMT, kNT, true>(p, ctas, st) : launch<kMT, kNT, false>(p, ctas, st);
 }
 
 template <int kMT>
-int dispatch_rank(const AdapterArgs &p, int ctas, bool fp32, bool vec, cudaStream_t st) {
-    if (p.rank <= 16) return dispatch_y<kMT, 2>(p, ctas, fp32, vec, st);
-    if (p.rank <= 32) return dispatch_y<kMT, 4>(p, ctas, fp32, vec, st);
-    if (p.rank <= 64) return dispatch_y<kMT, 8>(p, ctas, fp32, vec, st);
-    return dispatch_y<kMT, 16>(p, ctas, fp32, vec, st);
+int dispatch_rank(const AdapterArgs &p, int ctas, bool fp32, cudaStream_t st) {
+    if (p.rank <= 16) return dispatch_y<kMT, 2>(p, ctas, fp32, st);
+    if (p.rank <= 32) return dispatch_y<kMT, 4>(p, ctas, fp32, st);
+    if (p.rank <= 64) return dispatch_y<kMT, 8>(p, ctas, fp32, st);
+    return dispatch_y<kMT, 16>(p, ctas, fp32, st);
 }
 
 }  // namespace
@@ -363,20 +480,21 @@ extern "C" int moe_adapter_add(const void *x, int T, int K, int N, const void *a
         overlap(out, ny, scale, (size_t)adapters * 4) || overlap(out, ny, ids, (size_t)T * 4))
         return moe_set_error(MOE_EINVAL, "adapters: out may be y itself, but not overlap it or another input");
     AdapterArgs p{static_cast<const uint16_t *>(x), T, K, N, static_cast<const uint16_t *>(a),
-                  static_cast<const uint16_t *>(b), scale, adapters, rank, ids, y, out, 16, 1};
-    int ctas = kMaxCluster;
-    const bool vec = (ya & 15) == 0 && ((size_t)N * es) % 16 == 0;
-    const bool wide = T >= 512;
-    if (wide) {
-        p.rows = 64;
-        ctas = 4;
-    } else {
-        // enough clusters for all SMs: split N while a warp keeps a group, then take fewer rows a tile
-        const int tiles = (T + 15) / 16, want = 37;
-        while (p.splits * tiles < want && N / (p.splits + 1) >= ctas * kWarps * kGroup) ++p.splits;
-        const int rows = (int)(((long long)T * p.splits * ctas + 147) / 148);
-        p.rows = rows < 16 ? rows : 16;
-    }
-    return wide ? dispatch_rank<4>(p, ctas, y_fp32 != 0, vec, as_stream(stream))
-                : dispatch_rank<1>(p, ctas, y_fp32 != 0, vec, as_stream(stream));
+                  static_cast<const uint16_t *>(b), scale, adapters, rank, ids, y, out, 16, 1, 0,
+                  (ya & 15) == 0 && ((size_t)N * es) % 16 == 0};
+    // Rows a tile: as few as leave two CTAs an SM at four CTAs a tile, since the phases of a tile follow
+    // one another and only more tiles hide that (64 rows of 48 adapters, K = 3,072, N = 768: 6.6 us with
+    // one row a tile, 8.2 with two, 10 with four; 2,048 rows of rank 64: 26 us with 32, 31 with 16). A wide
+    // N (an LM head) is split over clusters of two, which repeat the small first product.
+    const int full = 296;              // two CTAs on each of 148 SMs
+    p.rows = 1;
+    while (p.rows < 32 && (long long)((T + p.rows - 1) / p.rows) * 4 > full) p.rows *= 2;
+    const int tiles = (T + p.rows - 1) / p.rows;
+    int ctas = tiles * 8 <= full ? kMaxCluster : tiles * 4 <= 2 * full ? 4 : 2;
+    if (N >= 16384) ctas = 2;
+    while (tiles * ctas * (p.splits + 1) <= full && N / (ctas * (p.splits + 1)) >= kWarps * 64) ++p.splits;
+    const bool wide = p.rows > 16;
+    p.sort = p.rows > 1 && T > p.rows && adapters <= kMaxSort;
+    return wide ? dispatch_rank<2>(p, ctas, y_fp32 != 0, as_stream(stream))
+                : dispatch_rank<1>(p, ctas, y_fp32 != 0, as_stream(stream));
 }
