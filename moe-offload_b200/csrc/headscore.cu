@@ -4,9 +4,11 @@
 //   score_kernel   the product X . W^T on the tensor cores: a pair of CTAs (tcgen05 cta_group::2) makes
 //                  a tile of 256 rows x up to 256 vocabulary entries, fp32 accumulators in TMEM, and
 //                  consumes it where it lies: every row keeps its running softmax statistics
-//                  (toplist.cuh) and a list of its largest logits. A pair stays with one block of
-//                  256 rows and walks every P-th vocabulary tile; pairs of different row blocks walk
-//                  the same tiles side by side, so the head is read from HBM once and from L2 after that.
+//                  and a list of its largest logits. A pair stays with one block of 256 rows and walks
+//                  every P-th vocabulary tile; pairs of different row blocks walk the same tiles side
+//                  by side, so the head is read from HBM once and from L2 after that. Up to 128 rows,
+//                  where the head's bytes are the bound, every CTA works alone on tiles of 128 rows: a
+//                  pair would take twice as long for the same bytes.
 //   finish_kernel  one CTA per row: joins the parts, sums the leading candidates' and the target's
 //                  logits again in 64 bits, exactly as the LM head does, corrects the statistics by
 //                  them and orders the alternatives.
@@ -33,35 +35,45 @@ namespace {
 constexpr int kM = 128;                // rows of X per CTA (TMEM lanes); a pair's MMA has M = 256
 constexpr int kN = 256;                // vocabulary entries per tile, at most (MMA N)
 constexpr int kK = 64;                 // K per stage: 128 bytes, the swizzle's width
-constexpr int kStages = 6;
 constexpr int kThreads = 320;          // TMA warp, MMA warp, 8 epilogue warps
 constexpr int kEpiWarps = 8;           // each 32 rows (its TMEM lanes) x half of the columns
 constexpr int kHalves = 2;
-constexpr uint32_t kABytes = kM * 128, kStageBytes = kABytes + kN / 2 * 128;       // (each CTA holds half of W's rows)
+constexpr uint32_t kABytes = kM * 128;
 constexpr uint32_t kTmemCols = 512;    // two accumulators of kN columns: one fills while one is read
 
-constexpr int kSlots = 64;             // a row's list in one part: what is kept, and room to append to
+constexpr int kSlots = 64;             // a row's list in one part
 constexpr int kPad = 8;                // kept beyond n, to tell whether the order of the n is settled
 constexpr int kKeep = kTopMax + kPad;  // at most
-constexpr int kSpare = 4;
+constexpr int kBins = 64;              // disjoint maxima of a row, for a bound on its keep-th largest logit
 constexpr int kMaxGroup = 8;           // 256-row blocks per launch: 74 / 8 = 9 parts, 144 of 148 CTAs busy
 constexpr float kMargin = 16.f;
 
 struct ScoreArgs {
     int T, V, H;                       // rows of this launch
-    int blocks, parts;                 // 256-row blocks, vocabulary parts (pairs = blocks * parts)
-    int width;                         // vocabulary entries per tile
+    int blocks, parts;                 // row blocks (256 or 128 rows), vocabulary parts
+    int width, xbox;                   // vocabulary entries per tile, rows of X per load
     int keep;                          // entries a list has to keep
     uint2 *lists;                      // [128-row blocks][parts][kHalves][kSlots][kM] (value, index)
     float4 *stats;                     // [128-row blocks][parts][kHalves][kM] m, s, w, entries (as int bits)
+    unsigned *bins;                    // [128-row blocks][kBins][kM] order images of maxima, 0 before the launch
     int *redo;                         // [0]: rows for exact_kernel
 };
 
+template <bool kPair>
 struct ScoreSmem {
+    static constexpr int kStages = kPair ? 6 : 4;
+    static constexpr uint32_t kStageBytes = kABytes + (kPair ? kN / 2 : kN) * 128; // (a pair's CTAs hold half of W each)
     static constexpr size_t bars = (size_t)kStages * kStageBytes;
     // full, empty [kStages]; acc_full, acc_empty [2]; drain; TMEM slot, abort flag
     static constexpr size_t alloc = bars + (2 * kStages + 5) * 8 + 16 + 1024;
 };
+
+MOE_D void mma_bf16_ss(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
 
 // ---- pair forms (cta_group::2): the CTA of rank 0 issues for both, its barriers collect both CTAs'
 // loads and both CTAs' epilogues
@@ -134,26 +146,32 @@ MOE_D uint32_t order_of(float f) {
 
 MOE_D float value_of(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
 
-// Cuts a thread's list (more than keep + kSpare entries) down to its keep largest entries, or up to
-// kSpare more where that ends the search sooner. Equal entries that do not all fit stay lowest index
+// the largest float below an image's (the image between those of -1e-45 and +0 is that of -0, equal to +0)
+MOE_D float value_below(uint32_t o) { return value_of(o - (o == 0x80000000u ? 2u : 1u)); }
+
+// Cuts a thread's list (more than keep + spare entries) down to its keep largest entries, or up to
+// spare more where that ends the search sooner. Equal entries that do not all fit stay lowest index
 // first (the list is in index order, and stays so). Returns a value that at least keep of the kept
 // entries reach: what comes later and does not exceed it is not among the keep largest. The 32 rows of
 // a warp work side by side, each bisecting for its own bound by counting.
-MOE_D float list_cut(uint2 *list, int &count, int keep) {
+MOE_D float list_cut(uint2 *list, int &count, int keep, int spare) {
     uint32_t o[kSlots];
     uint32_t lo = 0xffffffffu, hi = 0u;
+    // (slots behind the list are read too, and left out)
 #pragma unroll
-    for (int i = 0; i < kSlots; ++i) o[i] = i < count ? order_of(__uint_as_float(list[i * kM].x)) : 0u;
+    for (int i = 0; i < kSlots; ++i) o[i] = list[i * kM].x;
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
+        o[i] = i < count ? order_of(__uint_as_float(o[i])) : 0u;
         hi = max(hi, o[i]);
-        lo = min(lo, o[i] ? o[i] : 0xffffffffu);
+        lo = min(lo, o[i] - 1u);                  // (0 - 1: the largest)
     }
     // at least keep entries reach lo, fewer reach hi
     int reach = count;
+    lo += 1u;
     hi += 1u;
 #pragma unroll 1
-    while (reach > keep + kSpare && hi - lo > 1u) {
+    while (reach > keep + spare && hi - lo > 1u) {
         const uint32_t mid = lo + (hi - lo) / 2u;
         int n = 0;
 #pragma unroll
@@ -166,22 +184,28 @@ MOE_D float list_cut(uint2 *list, int &count, int keep) {
         }
     }
     int ties = kSlots;                            // how many of those equal to lo stay
-    if (reach > keep + kSpare) {
+    if (reach > keep + spare) {
         ties = keep;
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) ties -= o[i] > lo ? 1 : 0;
     }
+    // 16 indices in flight while the 16 before are moved (down, so never onto those)
+    constexpr int kB = 16;
+    uint32_t id[2][kB];
     int at = 0;
 #pragma unroll
-    for (int i0 = 0; i0 < kSlots; i0 += 8) {      // 8 entries in flight (they are in L2)
-        uint2 e[8];
+    for (int i = 0; i < kB; ++i) id[0][i] = list[i * kM].y;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (o[i0 + i] >= lo) e[i] = list[(i0 + i) * kM];
+    for (int i0 = 0; i0 < kSlots; i0 += kB) {
+        if (i0 + kB < kSlots) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (o[i0 + i] > lo || (o[i0 + i] == lo && ties-- > 0)) {
-                list[at * kM] = e[i];
+            for (int i = 0; i < kB; ++i) id[(i0 / kB + 1) & 1][i] = list[(i0 + kB + i) * kM].y;
+        }
+#pragma unroll
+        for (int i = 0; i < kB; ++i) {
+            const uint32_t k = o[i0 + i];
+            if (k > lo || (k == lo && ties-- > 0)) {
+                list[at * kM] = make_uint2(__float_as_uint(value_of(k)), id[(i0 / kB) & 1][i]);
                 ++at;
             }
         }
@@ -190,12 +214,91 @@ MOE_D float list_cut(uint2 *list, int &count, int keep) {
     return value_of(lo);
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+// A row's statistics while its tiles go by, in steps of 2: sums over 2^(x log2(e) - r) with r a whole
+// number near log2(e) times the largest value m, which the sums leave out (as SoftRun does). r is exact,
+// rescaling by it too, and one FMA makes an exponent. The constant's own rounding moves e^x by |x| 2^-24,
+// alike for values alike, and so do its uses here: fine for logits up to some hundreds.
+struct Run2 {
+    float m, r, s, w;                  // w: sum of t 2^t, t the exponents
+};
+constexpr float kLog2e = 1.4426950408889634f;
+
+MOE_D float pow2(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 32 values, top their largest (NaN left out)
+MOE_D void run2_add(Run2 &a, const float (&x)[32], float top) {
+    float s[2] = {a.s, 0.f}, w[2] = {a.w, 0.f};
+    if (__any_sync(0xffffffffu, top > a.m)) {     // somebody's largest value changes
+        const float want = floorf(top * kLog2e);
+        if (top > a.m && !(want <= a.r + 40.f && a.m > -INFINITY)) {
+            const float d = a.m > -INFINITY ? fmaxf(a.r - want, kSoftFar) : 0.f, f = pow2(d);
+            w[0] = f * (w[0] + d * s[0]);
+            s[0] *= f;                            // (nothing in the sums yet: 0, or NaN)
+            a.r = want;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float t = fmaf(min_nan(a.m, x[i]), kLog2e, -a.r), e = pow2(t);
+            a.m = fmaxf(a.m, x[i]);
+            s[i & 1] += e;
+            w[i & 1] = fmaf(fmaxf(t, kSoftFar), e, w[i & 1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float t = fmaf(x[i], kLog2e, -a.r), e = pow2(t);
+            s[i & 1] += e;
+            w[i & 1] = fmaf(fmaxf(t, kSoftFar), e, w[i & 1]);
+        }
+    }
+    a.s = s[0] + s[1];
+    a.w = w[0] + w[1];
+}
+
+MOE_D Soft run2_end(const Run2 &a) {
+    if (a.m == -INFINITY) return Soft{a.m, a.s, 0.f};
+    const float ln2 = 0.6931471805599453f;
+    const float d = (float)((double)a.r * 0.6931471805599453 - (double)a.m), f = __expf(d);
+    return Soft{a.m, f * a.s, f * fmaf(ln2, a.w, d * a.s)};
+}
+
+// A bound that at least keep of the row's logits reach, from its maxima so far in kBins disjoint sets
+// of vocabulary entries (kM apart): their keep-th largest, or a little less. 0: fewer maxima than that.
+MOE_D uint32_t bins_bound(const uint32_t (&o)[kBins], int keep) {
+    uint32_t lo = 0u, hi = 0u;
+#pragma unroll
+    for (int i = 0; i < kBins; ++i) hi = max(hi, o[i]);
+    int reach = kBins;
+    hi += 1u;
+#pragma unroll 1
+    while (reach > keep + 2 && hi - lo > 1u) {
+        const uint32_t mid = lo + (hi - lo) / 2u;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kBins; ++i) n += o[i] >= mid ? 1 : 0;
+        if (n >= keep) {
+            lo = mid;
+            reach = n;
+        } else {
+            hi = mid;
+        }
+    }
+    return lo;
+}
+
+template <bool kPair>
+__global__ void __launch_bounds__(kThreads, 1)
     score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, ScoreArgs a) {
+    using SL = ScoreSmem<kPair>;
+    constexpr int kStages = SL::kStages, kCtas = kPair ? 2 : 1;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + ScoreSmem::bars);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + SL::bars);
     uint64_t *empty = full + kStages;
     uint64_t *acc_full = empty + kStages;
     uint64_t *acc_empty = acc_full + 2;
@@ -204,113 +307,145 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // set by the first failed wait of any role of the CTA: the others stop, and what was issued is drained
     volatile int *abort = reinterpret_cast<volatile int *>(tslot + 1);
     cg::cluster_group pair = cg::this_cluster();
-    const int rank = (int)pair.block_rank();
+    const int rank = kPair ? (int)pair.block_rank() : 0;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(&full[i], 1);              // (used in the first CTA)
+            mbar_init(&full[i], 1);              // (used in a pair's first CTA)
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 2 * kEpiWarps);             // (in the first CTA, by both)
+            mbar_init(&acc_empty[i], kCtas * kEpiWarps);         // (in the first CTA, by both)
         }
         mbar_init(drain, 1);
         *abort = 0;
         fence_barrier_init();
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (kPair) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (blockIdx.x == 0) *a.redo = 0;
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tslot)),
-                     "r"(kTmemCols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+        if (kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tslot)),
+                         "r"(kTmemCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tslot)),
+                         "r"(kTmemCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        }
     }
     tc_fence_before();
-    pair.sync();                                 // both CTAs' barriers are there
+    if (kPair) pair.sync();                      // both CTAs' barriers are there
+    else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tslot;
-    const int unit = blockIdx.x >> 1, block = unit % a.blocks, part = unit / a.blocks;
+    const int unit = blockIdx.x / kCtas, block = unit % a.blocks, part = unit / a.blocks;
     const int tiles = (a.V + a.width - 1) / a.width, nkb = (a.H + kK - 1) / kK;
 
-    if (warp == 0) {
-        // ---- TMA, in each CTA for its own shared memory: 128 rows of X and half of the tile's rows of W.
-        // Rows and columns outside the arrays arrive as zeros
-        const uint32_t bytes = 2u * (kABytes + (uint32_t)a.width * 64u);            // of both CTAs
-        uint32_t g = 0;
+    if (warp == 0 && lane == 0) {
+        // ---- TMA, one thread in each CTA for its own shared memory: 128 rows of X and the tile's rows of W (a
+        // pair: half of them). Rows and columns of a box outside the arrays arrive as zeros, which costs
+        // the TMA unit as much as data (one row in a box of 128 made the one-row case 1.4 times slower):
+        // a few rows come in boxes of 32, and rows of X in boxes wholly outside hold whatever was
+        // there, in lanes of the accumulator that nobody reads
+        const int row0 = (block * kCtas + rank) * kM;
+        auto boxes = [&](int r0) { return min(max((a.T - r0 + a.xbox - 1) / a.xbox, 0), kM / a.xbox); };
+        const int nx = boxes(row0), wrows = a.width / kCtas;
+        uint32_t bytes = (uint32_t)nx * a.xbox * 128u + (uint32_t)wrows * 128u;
+        if (kPair)                               // the first CTA's barrier counts both CTAs' bytes
+            bytes = (uint32_t)(boxes(block * 2 * kM) + boxes(block * 2 * kM + kM)) * a.xbox * 128u + (uint32_t)a.width * 128u;
+        uint32_t s = 0, phase = 1, g = 0;
         bool stop = false;
         for (int v = part; v < tiles && !stop; v += a.parts) {
-            for (int kb = 0; kb < nkb; ++kb, ++g) {
-                const int s = g % kStages;
-                if (!wait_or_abort(&empty[s], ((g / kStages) & 1u) ^ 1u, abort)) {
+            const int w0 = v * a.width + rank * wrows;
+            for (int x = 0; x < nkb * kK; x += kK) {
+                if (!wait_or_abort_thread(&empty[s], phase, abort)) {
                     stop = true;
                     break;
                 }
-                if (lane == 0) {
-                    unsigned char *st = smem + (size_t)s * kStageBytes;
+                unsigned char *st = smem + (size_t)s * SL::kStageBytes;
+                if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+                if (kPair) {
                     const uint32_t bar = first_cta_addr(&full[s]);
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-                    tma_load_2d_pair(st, &map_x, kb * kK, block * 2 * kM + rank * kM, bar);
-                    tma_load_2d_pair(st + kABytes, &map_w, kb * kK, v * a.width + rank * (a.width / 2), bar);
+                    tma_load_2d_pair(st + kABytes, &map_w, x, w0, bar);
+                    for (int i = 0; i < nx; ++i)
+                        tma_load_2d_pair(st + (size_t)i * a.xbox * 128, &map_x, x, row0 + i * a.xbox, bar);
+                } else {
+                    tma_load_2d(st + kABytes, &map_w, x, w0, &full[s]);
+                    for (int i = 0; i < nx; ++i)
+                        tma_load_2d(st + (size_t)i * a.xbox * 128, &map_x, x, row0 + i * a.xbox, &full[s]);
                 }
-                __syncwarp();
+                ++g;
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1u;
+                }
             }
         }
         // nothing may still arrive here when the CTA ends: the last round's releases (each follows the
         // loads and MMAs of its stage), or after an abort the loads themselves
-        if (!aborted(abort)) {
+        if (!*abort) {
             for (uint32_t i = g > (uint32_t)kStages ? g - kStages : 0u; i < g; ++i)
-                if (!wait_or_abort(&empty[i % kStages], (i / kStages) & 1u, abort)) break;
+                if (!wait_or_abort_thread(&empty[i % kStages], (i / kStages) & 1u, abort)) break;
         } else if (rank == 0) {
             for (uint32_t i = g > (uint32_t)kStages ? g - kStages : 0u; i < g; ++i)
                 mbar_wait(&full[i % kStages], (i / kStages) & 1u);
         }
-    } else if (warp == 1) {
-        // ---- MMA: one thread of the first CTA issues for both
-        const uint32_t idesc = instr_desc_bf16(2 * kM, a.width);
-        uint32_t g = 0, it = 0;
-        bool stop = rank != 0, issued = false;
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        // ---- MMA: one thread issues (of the first CTA, for both)
+        const uint32_t idesc = instr_desc_bf16(kCtas * kM, a.width);
+        uint32_t s = 0, phase = 0, it = 0;
+        bool stop = false, issued = false;
         for (int v = part; v < tiles && !stop; v += a.parts, ++it) {
             const uint32_t b = it & 1u;
-            if (aborted(abort) || !wait_or_abort(&acc_empty[b], ((it >> 1) & 1u) ^ 1u, abort)) break;
+            if (!wait_or_abort_thread(&acc_empty[b], ((it >> 1) & 1u) ^ 1u, abort)) break;
             tc_fence_after();
-            for (int kb = 0; kb < nkb; ++kb, ++g) {
-                const int s = g % kStages;
-                if (!wait_or_abort(&full[s], (g / kStages) & 1u, abort)) {
+            for (int kb = 0; kb < nkb; ++kb) {
+                if (!wait_or_abort_thread(&full[s], phase, abort)) {
                     stop = true;
                     break;
                 }
                 tc_fence_after();
-                if (lane == 0) {
-                    const uint64_t da = desc_sw128(smem_addr(smem + (size_t)s * kStageBytes));
-                    const uint64_t db = desc_sw128(smem_addr(smem + (size_t)s * kStageBytes + kABytes));
+                const uint64_t da = desc_sw128(smem_addr(smem + (size_t)s * SL::kStageBytes));
+                const uint64_t db = desc_sw128(smem_addr(smem + (size_t)s * SL::kStageBytes + kABytes));
 #pragma unroll
-                    for (int j = 0; j < kK / 16; ++j)
-                        mma_bf16_pair(tmem + b * kN, da + 2u * j, db + 2u * j, idesc, (kb | j) ? 1u : 0u);
-                    mma_commit_pair(&empty[s]);
+                for (int j = 0; j < kK / 16; ++j) {
+                    if (kPair) mma_bf16_pair(tmem + b * kN, da + 2u * j, db + 2u * j, idesc, (kb | j) ? 1u : 0u);
+                    else mma_bf16_ss(tmem + b * kN, da + 2u * j, db + 2u * j, idesc, (kb | j) ? 1u : 0u);
                 }
+                if (kPair) mma_commit_pair(&empty[s]);
+                else mma_commit(&empty[s]);
                 issued = true;
-                __syncwarp();
+                if (++s == (uint32_t)kStages) {
+                    s = 0;
+                    phase ^= 1u;
+                }
             }
             if (stop) break;
-            if (lane == 0) mma_commit_pair(&acc_full[b]);
-            __syncwarp();
+            if (kPair) mma_commit_pair(&acc_full[b]);
+            else mma_commit(&acc_full[b]);
         }
-        if (aborted(abort) && issued) {
-            if (lane == 0) mma_commit_pair_local(drain);
-            __syncwarp();
+        if (*abort && issued) {
+            if (kPair) mma_commit_pair_local(drain);
+            else mma_commit(drain);
             mbar_wait(drain, 0);
         }
-    } else {
+    } else if (warp >= 2) {
         // ---- epilogue: thread = row, the tile's columns 0 .. 127 or the rest
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const int cols = half ? a.width - kN / 2 : min(a.width, kN / 2);
-        const int mblock = block * 2 + rank, lrow = quarter * 32 + lane, row = mblock * kM + lrow;
+        const int mblock = block * kCtas + rank, lrow = quarter * 32 + lane, row = mblock * kM + lrow;
         const int slice = (mblock * a.parts + part) * kHalves + half;
         uint2 *list = a.lists + (size_t)slice * kSlots * kM + lrow;
+        unsigned *bins = a.bins + (size_t)mblock * kBins * kM + lrow;
         const bool any = mblock * kM + quarter * 32 < a.T;          // a row of this warp is there
-        SoftRun run = run_none();
+        const int spare = max((kSlots - 16 - a.keep) / 2, 4);
+        Run2 run{-INFINITY, 0.f, 0.f, 0.f};
         float least = row < a.T ? -INFINITY : INFINITY;              // appended: what is above it
+        float tops[kN / 2 / 32], told[kN / 2 / 32];                  // of the four sets of 32 columns; last told
+#pragma unroll
+        for (int j = 0; j < kN / 2 / 32; ++j) tops[j] = told[j] = -INFINITY;
         int count = 0;
         uint32_t it = 0;
         for (int v = part; v < tiles; v += a.parts, ++it) {
@@ -319,57 +454,100 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tc_fence_after();
             const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + b * kN + half * (kN / 2);
             const int col0 = v * a.width + half * (kN / 2);
-            if (any) {
-#pragma unroll 1
-                for (int c = 0; c < cols; c += 32) {
-                    float q[32];
-                    tmem_ld32(taddr + c, q);
-                    const int col = col0 + c;
-                    if (col + 32 > a.V) {
+            const int inside = min(cols, a.V - col0);               // columns that are there
+            auto load = [&](int c, float (&x)[32]) {
+                tmem_ld32(taddr + c, x);
+                if (c + 32 > inside) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (col + i >= a.V) q[i] = -INFINITY;
+                    for (int i = 0; i < 32; ++i)
+                        if (c + i >= inside) x[i] = -INFINITY;
+                }
+            };
+            if (any && inside > 0) {
+                // After 0, 1, 2, 4, 8, .. tiles the row's parts tell each other their maxima, and each takes a
+                // bound on what is worth a place in its list from them (a look at the first tile comes
+                // before everything else). It may miss what others have just told: any such bound
+                // is a valid one, and the entries above the last are there in any case.
+                if ((it & (it - 1u)) == 0u) {
+                    if (it == 0) {
+#pragma unroll
+                        for (int j = 0; j < kN / 2 / 32; ++j) {
+                            if (32 * j < inside) {
+                                float x[32];
+                                load(32 * j, x);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) tops[j] = fmaxf(tops[j], x[i]);
+                            }
+                        }
                     }
+                    if (row < a.T) {
 #pragma unroll
-                    for (int h = 0; h < 32; h += 16) {
-                        float x[16];
+                        for (int j = 0; j < kN / 2 / 32; ++j) {
+                            if (tops[j] > told[j])
+                                atomicMax(&bins[(((part * kHalves + half) * 4 + j) % kBins) * kM], order_of(tops[j] + 0.f));
+                            told[j] = tops[j];
+                        }
+                    }
+                    uint32_t o[kBins];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) x[i] = q[h + i] + 0.f;
-                        float top = x[0];
+                    for (int i = 0; i < kBins; ++i) o[i] = __ldcg(&bins[i * kM]);
+                    const uint32_t bound = bins_bound(o, a.keep);
+                    // (entries equal to the bound may belong: they are settled by index)
+                    if (row < a.T && bound > 2u) least = fmaxf(least, value_below(bound));
+                }
 #pragma unroll
-                        for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
-                        if (__any_sync(0xffffffffu, top > least)) {
+                for (int j = 0; j < kN / 2 / 32; ++j) {
+                    if (32 * j >= inside) break;
+                    float x[32];
+                    load(32 * j, x);
+                    float top[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        top[h] = x[16 * h];
+#pragma unroll
+                        for (int i = 1; i < 16; ++i) top[h] = fmaxf(top[h], x[16 * h + i]);
+                        if (__any_sync(0xffffffffu, top[h] > least)) {
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
-                                if (x[i] > least) {
-                                    list[count * kM] = make_uint2(__float_as_uint(x[i]), (uint32_t)(col + h + i));
+                                if (x[16 * h + i] > least) {                        // (+ 0: no -0 in a list)
+                                    list[count * kM] = make_uint2(__float_as_uint(x[16 * h + i] + 0.f),
+                                                                  (uint32_t)(col0 + 32 * j + 16 * h + i));
                                     ++count;
                                 }
                             }
                             if (__any_sync(0xffffffffu, count > kSlots - 16)) {
-                                if (count > a.keep + kSpare) least = list_cut(list, count, a.keep);
+                                if (count > a.keep + spare) least = fmaxf(least, list_cut(list, count, a.keep, spare));
                                 __syncwarp();
                             }
                         }
-                        run_add(run, x, top);
                     }
+                    tops[j] = fmaxf(tops[j], fmaxf(top[0], top[1]));
+                    run2_add(run, x, fmaxf(top[0], top[1]));
                 }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) arrive_first_cta(first_cta_addr(&acc_empty[b]));
+            if (lane == 0) {
+                if (kPair) arrive_first_cta(first_cta_addr(&acc_empty[b]));
+                else mbar_arrive(&acc_empty[b]);
+            }
         }
         if (row < a.T) {
-            const Soft s = run_end(run);
+            const Soft s = run2_end(run);
             a.stats[(size_t)slice * kM + lrow] = make_float4(s.m, s.s, s.w, __int_as_float(count));
         }
     }
     __syncwarp();
     tc_fence_before();
-    pair.sync();                                 // neither CTA's memory goes while the other may reach it
+    if (kPair) pair.sync();                      // neither CTA's memory goes while the other may reach it
+    else __syncthreads();
     tc_fence_after();
-    if (warp == 1)
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    if (warp == 1) {
+        if (kPair)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    }
 }
 
 // ------------------------------------------------------------------ exact logits
@@ -642,23 +820,47 @@ __global__ void __cluster_dims__(kExCluster, 1, 1) __launch_bounds__(kExThreads)
 }
 
 struct Plan {
-    int pairs, sms;                    // CTA pairs that run at once
-    size_t lists, stats, redo, bytes;  // offsets
+    int sms;
+    bool paired;                       // 256-row blocks by CTA pairs, or one of 128 rows
+    size_t lists, stats, bins, redo, bytes;    // offsets
 };
 
 int make_plan(int T, Plan &pl) {
     int dev = 0;
     MOE_CUDA_TRY(cudaGetDevice(&dev));
     MOE_CUDA_TRY(cudaDeviceGetAttribute(&pl.sms, cudaDevAttrMultiProcessorCount, dev));
-    pl.pairs = pl.sms / 2;
-    if (pl.pairs < kMaxGroup)
+    if (pl.sms < 2 * kMaxGroup)
         return moe_set_error(MOE_ENODEV, "head logprobs: a device of %d SMs (%d needed)", pl.sms, 2 * kMaxGroup);
-    const size_t slices = (size_t)pl.pairs * 2 * kHalves;          // blocks * parts <= pairs in every launch
+    pl.paired = T > kM;
+    // 128-row blocks x parts is at most the number of SMs in every launch
+    const size_t slices = (size_t)pl.sms * kHalves;
     const int rows = T < kMaxGroup * 2 * kM ? T : kMaxGroup * 2 * kM;
+    const size_t mblocks = pl.paired ? 2 * (((size_t)rows + 2 * kM - 1) / (2 * kM)) : 1;
     pl.lists = 0;
     pl.stats = al256(slices * kSlots * kM * sizeof(uint2));
-    pl.redo = pl.stats + al256(slices * kM * sizeof(float4));
+    pl.bins = pl.stats + al256(slices * kM * sizeof(float4));
+    pl.redo = pl.bins + al256(mblocks * kBins * kM * sizeof(unsigned));
     pl.bytes = pl.redo + al256((1 + 3 * (size_t)rows) * sizeof(int));
+    return MOE_OK;
+}
+
+template <bool kPair>
+int launch_score(const CUtensorMap &mx, const CUtensorMap &mw, const ScoreArgs &a, cudaStream_t st) {
+    auto kern = score_kernel<kPair>;
+    const size_t smem = ScoreSmem<kPair>::alloc;
+    MOE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.blocks * a.parts * (kPair ? 2 : 1)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kPair ? 2 : 1;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mx, mw, a));
     return MOE_OK;
 }
 
@@ -688,18 +890,18 @@ extern "C" int moe_head_logprobs(const void *head, int V, int H, const void *x, 
     float4 *stats = reinterpret_cast<float4 *>(ws + pl.stats);
     int *redo = reinterpret_cast<int *>(ws + pl.redo);
     cudaStream_t st = as_stream(stream);
+    unsigned *bins = reinterpret_cast<unsigned *>(ws + pl.bins);
     CUtensorMap mw, mx;
     int rc;
-    MOE_CUDA_TRY(cudaFuncSetAttribute(score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ScoreSmem::alloc));
     for (int t0 = 0; t0 < T; t0 += kMaxGroup * 2 * kM) {
         const int rows = T - t0 < kMaxGroup * 2 * kM ? T - t0 : kMaxGroup * 2 * kM;
-        const int blocks = (rows + 2 * kM - 1) / (2 * kM);
-        int parts = pl.pairs / blocks;
-        // the tile width that leaves the busiest pair the fewest entries (V = 248,320 over 74 parts: 14 tiles of
-        // 256, or 15 of 224, 6 % less)
+        const int ctas = pl.paired ? 2 : 1, blocks = (rows + ctas * kM - 1) / (ctas * kM);
+        int parts = pl.sms / ctas / blocks;
+        // the tile width that leaves the busiest part the fewest entries (V = 248,320 over 148 parts: 7 tiles of
+        // 256, or 7 of 240, 6 % less)
         int width = kN;
         long long most = -1;
-        for (int w = kN; w >= 192; w -= 32) {
+        for (int w = kN; w >= 192; w -= 16 * ctas) {
             const int tiles = (V + w - 1) / w;
             const long long m = (long long)((tiles + parts - 1) / parts) * w;
             if (most < 0 || m < most) {
@@ -708,15 +910,17 @@ extern "C" int moe_head_logprobs(const void *head, int V, int H, const void *x, 
             }
         }
         if (parts > (V + width - 1) / width) parts = (V + width - 1) / width;
+        const int xbox = rows >= kM ? kM : 32;
         const uint16_t *xr = static_cast<const uint16_t *>(x) + (size_t)t0 * H;
         rc = make_map("head logprobs", &mw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, head, (uint64_t)H, (uint64_t)V, kK,
-                      (uint32_t)width / 2);
+                      (uint32_t)(width / ctas));
         if (!rc)
-            rc = make_map("head logprobs", &mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, xr, (uint64_t)H, (uint64_t)rows, kK, kM);
+            rc = make_map("head logprobs", &mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, xr, (uint64_t)H, (uint64_t)rows, kK,
+                          (uint32_t)xbox);
         if (rc) return rc;
-        const ScoreArgs sa{rows, V, H, blocks, parts, width, n + kPad, lists, stats, redo};
-        score_kernel<<<blocks * parts * 2, kThreads, ScoreSmem::alloc, st>>>(mx, mw, sa);
-        MOE_CUDA_TRY(cudaGetLastError());
+        const ScoreArgs sa{rows, V, H, blocks, parts, width, xbox, n + kPad, lists, stats, bins, redo};
+        MOE_CUDA_TRY(cudaMemsetAsync(bins, 0, (size_t)blocks * ctas * kBins * kM * sizeof(unsigned), st));
+        if ((rc = pl.paired ? launch_score<true>(mx, mw, sa, st) : launch_score<false>(mx, mw, sa, st))) return rc;
         int32_t *ids = n ? top_ids + (size_t)t0 * n : nullptr;
         float *tl = n ? top_logprobs + (size_t)t0 * n : nullptr;
         const FinishArgs fa{static_cast<const uint16_t *>(head), xr, V, H, n, parts, n + kPad, lists, stats,

@@ -59,6 +59,18 @@ MOE_D bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort) {
     return ok;
 }
 
+// The same for one thread alone (a producer or issuer that its warp does not wait with).
+MOE_D bool wait_or_abort_thread(uint64_t *bar, uint32_t parity, volatile int *abort) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kMbarSpinLimit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 1023u) == 1023u && *abort) return false;
+    }
+    atomicOr(&g_moe_device_error, MOE_DEVERR_MBAR_TIMEOUT);
+    *abort = 1;
+    return false;
+}
+
 MOE_D bool aborted(volatile int *abort) { return __any_sync(0xffffffffu, *abort != 0); }
 
 // 2-D tiled TMA load (no multicast) completing on an mbarrier; x is the innermost coordinate
