@@ -146,15 +146,17 @@ MOE_D uint32_t order_of(float f) {
 
 MOE_D float value_of(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
 
-// the largest float below an image's (the image between those of -1e-45 and +0 is that of -0, equal to +0)
-MOE_D float value_below(uint32_t o) { return value_of(o - (o == 0x80000000u ? 2u : 1u)); }
+// the largest float below an image's (the image between those of -1e-45 and +0 is that of -0, equal to
+// +0); -inf for none
+MOE_D float value_below(uint32_t o) { return o > 0x00800000u ? value_of(o - (o == 0x80000000u ? 2u : 1u)) : -INFINITY; }
 
 // Cuts a thread's list (more than keep + spare entries) down to its keep largest entries, or up to
 // spare more where that ends the search sooner. Equal entries that do not all fit stay lowest index
 // first (the list is in index order, and stays so). Returns a value that at least keep of the kept
 // entries reach: what comes later and does not exceed it is not among the keep largest. The 32 rows of
 // a warp work side by side, each bisecting for its own bound by counting.
-MOE_D float list_cut(uint2 *list, int &count, int keep, int spare) {
+// (Not inlined: it is hardly ever called, and its registers would spill those of the common path.)
+__device__ __noinline__ float list_cut(uint2 *list, int &count, int keep, int spare) {
     uint32_t o[kSlots];
     uint32_t lo = 0xffffffffu, hi = 0u;
     // (slots behind the list are read too, and left out)
@@ -221,28 +223,20 @@ MOE_D float list_cut(uint2 *list, int &count, int keep, int spare) {
 struct Run2 {
     float m, r, s, w;                  // w: sum of t 2^t, t the exponents
 };
-constexpr float kLog2e = 1.4426950408889634f;
-
-MOE_D float pow2(float x) {
-    float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // 32 values, top their largest (NaN left out)
 MOE_D void run2_add(Run2 &a, const float (&x)[32], float top) {
     float s[2] = {a.s, 0.f}, w[2] = {a.w, 0.f};
     if (__any_sync(0xffffffffu, top > a.m)) {     // somebody's largest value changes
         const float want = floorf(top * kLog2e);
         if (top > a.m && !(want <= a.r + 40.f && a.m > -INFINITY)) {
-            const float d = a.m > -INFINITY ? fmaxf(a.r - want, kSoftFar) : 0.f, f = pow2(d);
+            const float d = a.m > -INFINITY ? fmaxf(a.r - want, kSoftFar) : 0.f, f = fast_pow2(d);
             w[0] = f * (w[0] + d * s[0]);
             s[0] *= f;                            // (nothing in the sums yet: 0, or NaN)
             a.r = want;
         }
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float t = fmaf(min_nan(a.m, x[i]), kLog2e, -a.r), e = pow2(t);
+            const float t = fmaf(min_nan(a.m, x[i]), kLog2e, -a.r), e = fast_pow2(t);
             a.m = fmaxf(a.m, x[i]);
             s[i & 1] += e;
             w[i & 1] = fmaf(fmaxf(t, kSoftFar), e, w[i & 1]);
@@ -250,7 +244,7 @@ MOE_D void run2_add(Run2 &a, const float (&x)[32], float top) {
     } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float t = fmaf(x[i], kLog2e, -a.r), e = pow2(t);
+            const float t = fmaf(x[i], kLog2e, -a.r), e = fast_pow2(t);
             s[i & 1] += e;
             w[i & 1] = fmaf(fmaxf(t, kSoftFar), e, w[i & 1]);
         }
@@ -262,7 +256,7 @@ MOE_D void run2_add(Run2 &a, const float (&x)[32], float top) {
 MOE_D Soft run2_end(const Run2 &a) {
     if (a.m == -INFINITY) return Soft{a.m, a.s, 0.f};
     const float ln2 = 0.6931471805599453f;
-    const float d = (float)((double)a.r * 0.6931471805599453 - (double)a.m), f = __expf(d);
+    const float d = (float)((double)a.r * 0.6931471805599453 - (double)a.m), f = fast_exp(d);
     return Soft{a.m, f * a.s, f * fmaf(ln2, a.w, d * a.s)};
 }
 
@@ -275,7 +269,7 @@ MOE_D uint32_t bins_bound(const uint32_t (&o)[kBins], int keep) {
     int reach = kBins;
     hi += 1u;
 #pragma unroll 1
-    while (reach > keep + 2 && hi - lo > 1u) {
+    while (reach > keep + 6 && hi - lo > 1u) {
         const uint32_t mid = lo + (hi - lo) / 2u;
         int n = 0;
 #pragma unroll
@@ -450,8 +444,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t it = 0;
         for (int v = part; v < tiles; v += a.parts, ++it) {
             const uint32_t b = it & 1u;
+            // Before tiles 1, 2, 4, 8, .. each part takes a bound on what is worth a place in its list from
+            // the row's maxima that the parts have told each other (and before the first one, below). It may
+            // miss what others have just told: any such bound is a valid one, and the entries above
+            // the last are there in any case. The loads go out before the tile is there.
+            const bool look = any && it > 0 && (it & (it - 1u)) == 0u;
+            uint32_t o[kBins];
+            if (look) {
+#pragma unroll
+                for (int i = 0; i < kBins; ++i) o[i] = __ldcg(&bins[i * kM]);
+            }
             if (aborted(abort) || !wait_or_abort(&acc_full[b], (it >> 1) & 1u, abort)) break;
             tc_fence_after();
+            if (look) least = fmaxf(least, value_below(bins_bound(o, a.keep)));
             const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + b * kN + half * (kN / 2);
             const int col0 = v * a.width + half * (kN / 2);
             const int inside = min(cols, a.V - col0);               // columns that are there
@@ -463,67 +468,69 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (c + i >= inside) x[i] = -INFINITY;
                 }
             };
-            if (any && inside > 0) {
-                // After 0, 1, 2, 4, 8, .. tiles the row's parts tell each other their maxima, and each takes a
-                // bound on what is worth a place in its list from them (a look at the first tile comes
-                // before everything else). It may miss what others have just told: any such bound
-                // is a valid one, and the entries above the last are there in any case.
-                if ((it & (it - 1u)) == 0u) {
-                    if (it == 0) {
-#pragma unroll
-                        for (int j = 0; j < kN / 2 / 32; ++j) {
-                            if (32 * j < inside) {
-                                float x[32];
-                                load(32 * j, x);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) tops[j] = fmaxf(tops[j], x[i]);
-                            }
-                        }
-                    }
-                    if (row < a.T) {
-#pragma unroll
-                        for (int j = 0; j < kN / 2 / 32; ++j) {
-                            if (tops[j] > told[j])
-                                atomicMax(&bins[(((part * kHalves + half) * 4 + j) % kBins) * kM], order_of(tops[j] + 0.f));
-                            told[j] = tops[j];
-                        }
-                    }
-                    uint32_t o[kBins];
-#pragma unroll
-                    for (int i = 0; i < kBins; ++i) o[i] = __ldcg(&bins[i * kM]);
-                    const uint32_t bound = bins_bound(o, a.keep);
-                    // (entries equal to the bound may belong: they are settled by index)
-                    if (row < a.T && bound > 2u) least = fmaxf(least, value_below(bound));
-                }
+            auto tell = [&]() {
+                if (row >= a.T) return;
 #pragma unroll
                 for (int j = 0; j < kN / 2 / 32; ++j) {
-                    if (32 * j >= inside) break;
-                    float x[32];
-                    load(32 * j, x);
-                    float top[2];
+                    if (tops[j] > told[j])
+                        atomicMax(&bins[(((part * kHalves + half) * 4 + j) % kBins) * kM], order_of(tops[j] + 0.f));
+                    told[j] = tops[j];
+                }
+            };
+            if (any && inside > 0) {
+                // the first tile: its maxima are told, its statistics taken while the others tell theirs, and
+                // its candidates only then. Passes: 0 statistics, 1 candidates, 2 both
+                if (it == 0) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        top[h] = x[16 * h];
+                    for (int j = 0; j < kN / 2 / 32; ++j) {
+                        if (32 * j < inside) {
+                            float x[32];
+                            load(32 * j, x);
 #pragma unroll
-                        for (int i = 1; i < 16; ++i) top[h] = fmaxf(top[h], x[16 * h + i]);
-                        if (__any_sync(0xffffffffu, top[h] > least)) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                if (x[16 * h + i] > least) {                        // (+ 0: no -0 in a list)
-                                    list[count * kM] = make_uint2(__float_as_uint(x[16 * h + i] + 0.f),
-                                                                  (uint32_t)(col0 + 32 * j + 16 * h + i));
-                                    ++count;
-                                }
-                            }
-                            if (__any_sync(0xffffffffu, count > kSlots - 16)) {
-                                if (count > a.keep + spare) least = fmaxf(least, list_cut(list, count, a.keep, spare));
-                                __syncwarp();
-                            }
+                            for (int i = 0; i < 32; ++i) tops[j] = fmaxf(tops[j], x[i]);
                         }
                     }
-                    tops[j] = fmaxf(tops[j], fmaxf(top[0], top[1]));
-                    run2_add(run, x, fmaxf(top[0], top[1]));
+                    tell();
                 }
+#pragma unroll 1
+                for (int pass = it == 0 ? 0 : 2; pass <= (it == 0 ? 1 : 2); ++pass) {
+                    if (pass == 1) {
+#pragma unroll
+                        for (int i = 0; i < kBins; ++i) o[i] = __ldcg(&bins[i * kM]);
+                        least = fmaxf(least, value_below(bins_bound(o, a.keep)));
+                    }
+#pragma unroll 1
+                    for (int j = 0; 32 * j < inside; ++j) {
+                        float x[32];
+                        load(32 * j, x);
+                        float top[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            top[h] = x[16 * h];
+#pragma unroll
+                            for (int i = 1; i < 16; ++i) top[h] = fmaxf(top[h], x[16 * h + i]);
+                            if (pass != 0 && __any_sync(0xffffffffu, top[h] > least)) {
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    if (x[16 * h + i] > least) {                    // (+ 0: no -0 in a list)
+                                        list[count * kM] = make_uint2(__float_as_uint(x[16 * h + i] + 0.f),
+                                                                      (uint32_t)(col0 + 32 * j + 16 * h + i));
+                                        ++count;
+                                    }
+                                }
+                                if (__any_sync(0xffffffffu, count > kSlots - 16)) {
+                                    if (count > a.keep + spare) least = fmaxf(least, list_cut(list, count, a.keep, spare));
+                                    __syncwarp();
+                                }
+                            }
+                        }
+                        const float both = fmaxf(top[0], top[1]);
+#pragma unroll
+                        for (int k = 0; k < kN / 2 / 32; ++k) tops[k] = fmaxf(tops[k], k == j ? both : -INFINITY);
+                        if (pass != 1) run2_add(run, x, both);
+                    }
+                }
+                if ((it & (it + 1u)) == 0u) tell();                  // the next tile looks
             }
             tc_fence_before();
             __syncwarp();
@@ -555,7 +562,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 // x as floats, k-major (xs[k][c] = x[8 c + k]): lane-consecutive chunks read consecutive words
 MOE_D void stage_row(const uint16_t *x, int H, float *xs) {
     const int nch = H / 8;
-    for (int i = threadIdx.x; i < H; i += blockDim.x) xs[(i & 7) * nch + (i >> 3)] = bf16_bits_to_f32(x[i]);
+    for (int c = threadIdx.x; c < nch; c += blockDim.x) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(x) + c);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            xs[(2 * k) * nch + c] = __uint_as_float(w[k] << 16);
+            xs[(2 * k + 1) * nch + c] = __uint_as_float(w[k] & 0xffff0000u);
+        }
+    }
 }
 
 // A warp's dot product of a head row with the staged row: the products (exact in fp32) summed in
@@ -601,6 +616,7 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
     extern __shared__ float xs[];                                   // [H], k-major
     __shared__ unsigned long long cand[kCand], lead[kKeep];
     __shared__ float peaks[kFinThreads], exact[kKeep + 1];
+    __shared__ int counts[kFinThreads];
     __shared__ Soft softs[kFinWarps];
     __shared__ float tau_s;
     __shared__ int ncand;
@@ -620,37 +636,43 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
     for (int l = tid; l < nlists; l += kFinThreads) {
         const float4 f = stats[(size_t)l * kM];
         st = soft_merge(st, Soft{f.x, f.y, f.z});
+        if (l < kFinThreads) {
+            peaks[l] = f.x;
+            counts[l] = min(max(__float_as_int(f.w), 0), kSlots);
+        }
     }
     st = soft_warp(st);
     if (lane == 0) softs[warp] = st;
+    __syncthreads();
 
     // the leading candidates: the keep-th largest of many disjoint maxima is a bound that keep entries
     // reach. With enough lists their own maxima do, and only the lists that reach the bound are read;
-    // else those of 64 groups of 8 threads
+    // else those of 64 groups of 8 threads, which hold the entries of 2 lists a warp
+    constexpr int kPer = kSlots / 32;
     const bool by_list = nlists >= 2 * p.keep && nlists <= kFinThreads;
     const int npeaks = by_list ? nlists : kFinThreads / 8;
-    auto entries = [&](float from, auto &&f) {
-        for (int l = warp; l < nlists; l += kFinWarps) {
-            const float4 s4 = stats[(size_t)l * kM];
-            if (s4.x < from) continue;
-            const int count = min(max(__float_as_int(s4.w), 0), kSlots);
-            const uint2 *e = lists + (size_t)l * kSlots * kM;
-            const bool a = lane < count, b = lane + 32 < count;
-            const uint2 ea = a ? e[lane * kM] : make_uint2(0u, 0u), eb = b ? e[(lane + 32) * kM] : make_uint2(0u, 0u);
-            if (a) f(ea);
-            if (b) f(eb);
-        }
+    uint2 held[2][kPer];
+    auto load_list = [&](int l, uint2 (&e)[kPer]) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            e[i] = l < nlists && lane + 32 * i < counts[l] ? lists[((size_t)l * kSlots + lane + 32 * i) * kM]
+                                                           : make_uint2(0xff800000u, 0u);          // -inf
     };
-    if (by_list) {
-        if (tid < nlists) peaks[tid] = stats[(size_t)tid * kM].x;
-    } else {
+    if (!by_list) {
         float top = -INFINITY;
-        entries(-INFINITY, [&](uint2 e) { top = fmaxf(top, __uint_as_float(e.x)); });
+        for (int l = warp; l < nlists; l += 2 * kFinWarps) {
+            load_list(l, held[0]);
+            load_list(l + kFinWarps, held[1]);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                top = fmaxf(top, fmaxf(__uint_as_float(held[0][i].x), __uint_as_float(held[1][i].x)));
+        }
 #pragma unroll
         for (int off = 4; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        __syncthreads();                                            // (the lists' maxima are no longer needed)
         if ((lane & 7) == 0) peaks[tid >> 3] = top;
+        __syncthreads();
     }
-    __syncthreads();
     if (tid < npeaks) {
         const float mine = peaks[tid];
         int r = 0;
@@ -661,12 +683,26 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
     st = soft_warp(lane < kFinWarps ? softs[lane] : soft_none());
     __syncthreads();
     const float tau = tau_s;
-    entries(tau, [&](uint2 e) {
-        if (__uint_as_float(e.x) >= tau) {
-            const int at = atomicAdd(&ncand, 1);
-            if (at < kCand) cand[at] = top_key(__uint_as_float(e.x), (int)e.y);
+    const bool one_round = nlists <= 2 * kFinWarps;                  // held still has all entries
+    for (int l = warp; l < nlists; l += 2 * kFinWarps) {
+        if (by_list || !one_round) {
+            const bool a = !by_list || peaks[l] >= tau;
+            const bool b = l + kFinWarps < nlists && (!by_list || peaks[l + kFinWarps] >= tau);
+            if (!a && !b) continue;
+            load_list(a ? l : nlists, held[0]);
+            load_list(b ? l + kFinWarps : nlists, held[1]);
         }
-    });
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const float value = __uint_as_float(held[h][i].x);
+                if (value >= tau && value > -INFINITY) {
+                    const int at = atomicAdd(&ncand, 1);
+                    if (at < kCand) cand[at] = top_key(value, (int)held[h][i].y);
+                }
+            }
+    }
     __syncthreads();
     const int all = ncand, have = min(all, kCand);
     for (int i = tid; i < have; i += kFinThreads) {
@@ -702,7 +738,7 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
             err = fmaxf(err, fabsf(x - near));
             if (i > 0) {
                 const float dx = fmaxf(x - sum.m, kSoftFar), dn = fmaxf(near - sum.m, kSoftFar);
-                const float ex = __expf(dx), en = __expf(dn);
+                const float ex = fast_exp(dx), en = fast_exp(dn);
                 sum.s += ex - en;
                 sum.w += dx * ex - dn * en;
             }
@@ -713,7 +749,7 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
             sum.w += __shfl_xor_sync(0xffffffffu, sum.w, off);
             err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, off));
         }
-        const float d = st.m - sum.m, f = __expf(d);
+        const float d = st.m - sum.m, f = fast_exp(d);
         sum.s = fmaxf(fmaf(f, st.s, sum.s), 0.f);
         sum.w += f * (st.w + d * st.s);
     } else {
@@ -829,8 +865,9 @@ int make_plan(int T, Plan &pl) {
     int dev = 0;
     MOE_CUDA_TRY(cudaGetDevice(&dev));
     MOE_CUDA_TRY(cudaDeviceGetAttribute(&pl.sms, cudaDevAttrMultiProcessorCount, dev));
-    if (pl.sms < 2 * kMaxGroup)
-        return moe_set_error(MOE_ENODEV, "head logprobs: a device of %d SMs (%d needed)", pl.sms, 2 * kMaxGroup);
+    if (pl.sms < 2 * kMaxGroup || pl.sms * kHalves > kFinThreads)
+        return moe_set_error(MOE_ENODEV, "head logprobs: a device of %d SMs (%d to %d)", pl.sms, 2 * kMaxGroup,
+                             kFinThreads / kHalves);
     pl.paired = T > kM;
     // 128-row blocks x parts is at most the number of SMs in every launch
     const size_t slices = (size_t)pl.sms * kHalves;
