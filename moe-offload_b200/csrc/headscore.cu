@@ -47,6 +47,7 @@ constexpr int kKeep = kTopMax + kPad;  // at most
 constexpr int kBins = 64;              // disjoint maxima of a row, for a bound on its keep-th largest logit
 constexpr int kMaxGroup = 8;           // 256-row blocks per launch: 74 / 8 = 9 parts, 144 of 148 CTAs busy
 constexpr float kMargin = 16.f;
+constexpr int kExCluster = 8, kMaxClusters = 32;       // exact_kernel: CTAs per cluster, clusters at most
 
 struct ScoreArgs {
     int T, V, H;                       // rows of this launch
@@ -56,7 +57,7 @@ struct ScoreArgs {
     uint2 *lists;                      // [128-row blocks][parts][kHalves][kSlots][kM] (value, index)
     float4 *stats;                     // [128-row blocks][parts][kHalves][kM] m, s, w, entries (as int bits)
     unsigned *bins;                    // [128-row blocks][kBins][kM] order images of maxima, 0 before the launch
-    int *redo;                         // [0]: rows for exact_kernel
+    int *redo;                         // [0]: rows for exact_kernel, then its counters
 };
 
 template <bool kPair>
@@ -302,7 +303,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int *abort = reinterpret_cast<volatile int *>(tslot + 1);
     cg::cluster_group pair = cg::this_cluster();
     const int rank = kPair ? (int)pair.block_rank() : 0;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);          // (known to be uniform)
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&full[i], 1);              // (used in a pair's first CTA)
@@ -316,7 +318,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         *abort = 0;
         fence_barrier_init();
         if (kPair) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (blockIdx.x == 0) *a.redo = 0;
+        if (blockIdx.x == 0)
+            for (int i = 0; i <= kMaxClusters; ++i) a.redo[i] = 0;
     }
     if (warp == 1) {
         if (kPair) {
@@ -337,9 +340,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int unit = blockIdx.x / kCtas, block = unit % a.blocks, part = unit / a.blocks;
     const int tiles = (a.V + a.width - 1) / a.width, nkb = (a.H + kK - 1) / kK;
 
-    if (warp == 0 && lane == 0) {
-        // ---- TMA, one thread in each CTA for its own shared memory: 128 rows of X and the tile's rows of W (a
-        // pair: half of them). Rows and columns of a box outside the arrays arrive as zeros, which costs
+    // The two control warps run in step with one lane elected to issue, and with the stages unrolled: beside
+    // eight busy epilogue warps their own instructions are what limits them (512 cycles a K block)
+    if (warp == 0) {
+        // ---- TMA, in each CTA for its own shared memory: 128 rows of X and the tile's rows of W (a pair: half of
+        // them). Rows and columns of a box outside the arrays arrive as zeros, which costs
         // the TMA unit as much as data (one row in a box of 128 made the one-row case 1.4 times slower):
         // a few rows come in boxes of 32, and rows of X in boxes wholly outside hold whatever was
         // there, in lanes of the accumulator that nobody reads
@@ -349,80 +354,108 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t bytes = (uint32_t)nx * a.xbox * 128u + (uint32_t)wrows * 128u;
         if (kPair)                               // the first CTA's barrier counts both CTAs' bytes
             bytes = (uint32_t)(boxes(block * 2 * kM) + boxes(block * 2 * kM + kM)) * a.xbox * 128u + (uint32_t)a.width * 128u;
-        uint32_t s = 0, phase = 1, g = 0;
-        bool stop = false;
-        for (int v = part; v < tiles && !stop; v += a.parts) {
-            const int w0 = v * a.width + rank * wrows;
-            for (int x = 0; x < nkb * kK; x += kK) {
-                if (!wait_or_abort_thread(&empty[s], phase, abort)) {
+        const uint32_t full0 = kPair ? first_cta_addr(full) : smem_addr(full);
+        const int kend = nkb * kK;
+        uint32_t phase = 1, g = 0;
+        int v = part, x = 0;
+        bool stop = v >= tiles;
+        while (!stop) {
+#pragma unroll
+            for (int s = 0; s < kStages; ++s) {
+                if (stop) continue;
+                if (!wait_or_abort_step(&empty[s], phase, abort)) {
                     stop = true;
-                    break;
+                    continue;
                 }
-                unsigned char *st = smem + (size_t)s * SL::kStageBytes;
-                if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-                if (kPair) {
-                    const uint32_t bar = first_cta_addr(&full[s]);
-                    tma_load_2d_pair(st + kABytes, &map_w, x, w0, bar);
-                    for (int i = 0; i < nx; ++i)
-                        tma_load_2d_pair(st + (size_t)i * a.xbox * 128, &map_x, x, row0 + i * a.xbox, bar);
-                } else {
-                    tma_load_2d(st + kABytes, &map_w, x, w0, &full[s]);
-                    for (int i = 0; i < nx; ++i)
-                        tma_load_2d(st + (size_t)i * a.xbox * 128, &map_x, x, row0 + i * a.xbox, &full[s]);
+                if (elect_lane()) {
+                    unsigned char *st = smem + (size_t)s * SL::kStageBytes;
+                    const int w0 = v * a.width + rank * wrows;
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+                    if (kPair) {
+                        tma_load_2d_pair(st + kABytes, &map_w, x, w0, full0 + 8u * s);
+                        for (int i = 0; i < nx; ++i)
+                            tma_load_2d_pair(st + (size_t)i * a.xbox * 128, &map_x, x, row0 + i * a.xbox, full0 + 8u * s);
+                    } else {
+                        tma_load_2d(st + kABytes, &map_w, x, w0, &full[s]);
+                        for (int i = 0; i < nx; ++i)
+                            tma_load_2d(st + (size_t)i * a.xbox * 128, &map_x, x, row0 + i * a.xbox, &full[s]);
+                    }
                 }
+                __syncwarp();
                 ++g;
-                if (++s == kStages) {
-                    s = 0;
-                    phase ^= 1u;
+                x += kK;
+                if (x >= kend) {
+                    x = 0;
+                    v += a.parts;
+                    stop = v >= tiles;
                 }
             }
+            phase ^= 1u;
         }
         // nothing may still arrive here when the CTA ends: the last round's releases (each follows the
         // loads and MMAs of its stage), or after an abort the loads themselves
-        if (!*abort) {
+        if (!aborted(abort)) {
             for (uint32_t i = g > (uint32_t)kStages ? g - kStages : 0u; i < g; ++i)
-                if (!wait_or_abort_thread(&empty[i % kStages], (i / kStages) & 1u, abort)) break;
+                if (!wait_or_abort_step(&empty[i % kStages], (i / kStages) & 1u, abort)) break;
         } else if (rank == 0) {
             for (uint32_t i = g > (uint32_t)kStages ? g - kStages : 0u; i < g; ++i)
                 mbar_wait(&full[i % kStages], (i / kStages) & 1u);
         }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        // ---- MMA: one thread issues (of the first CTA, for both)
+    } else if (warp == 1 && rank == 0) {
+        // ---- MMA (a pair's first CTA issues for both)
         const uint32_t idesc = instr_desc_bf16(kCtas * kM, a.width);
-        uint32_t s = 0, phase = 0, it = 0;
-        bool stop = false, issued = false;
-        for (int v = part; v < tiles && !stop; v += a.parts, ++it) {
-            const uint32_t b = it & 1u;
-            if (!wait_or_abort_thread(&acc_empty[b], ((it >> 1) & 1u) ^ 1u, abort)) break;
-            tc_fence_after();
-            for (int kb = 0; kb < nkb; ++kb) {
-                if (!wait_or_abort_thread(&full[s], phase, abort)) {
+        const uint64_t desc0 = desc_sw128(smem_addr(smem));         // (16-byte units in the low bits)
+        uint32_t phase = 0, it = 0;
+        int v = part, kb = 0;
+        bool stop = v >= tiles, issued = false;
+        while (!stop) {
+#pragma unroll
+            for (int s = 0; s < kStages; ++s) {
+                if (stop) continue;
+                const uint32_t b = it & 1u;
+                if (kb == 0 && !wait_or_abort_step(&acc_empty[b], ((it >> 1) & 1u) ^ 1u, abort)) {
                     stop = true;
-                    break;
+                    continue;
+                }
+                if (!wait_or_abort_step(&full[s], phase, abort)) {
+                    stop = true;
+                    continue;
                 }
                 tc_fence_after();
-                const uint64_t da = desc_sw128(smem_addr(smem + (size_t)s * SL::kStageBytes));
-                const uint64_t db = desc_sw128(smem_addr(smem + (size_t)s * SL::kStageBytes + kABytes));
+                const bool last = kb + 1 == nkb;
+                if (elect_lane()) {
+                    const uint64_t da = desc0 + (s * SL::kStageBytes) / 16u, db = da + kABytes / 16u;
+                    const uint32_t d = tmem + b * kN;
 #pragma unroll
-                for (int j = 0; j < kK / 16; ++j) {
-                    if (kPair) mma_bf16_pair(tmem + b * kN, da + 2u * j, db + 2u * j, idesc, (kb | j) ? 1u : 0u);
-                    else mma_bf16_ss(tmem + b * kN, da + 2u * j, db + 2u * j, idesc, (kb | j) ? 1u : 0u);
+                    for (int j = 0; j < kK / 16; ++j) {
+                        if (kPair) mma_bf16_pair(d, da + 2u * j, db + 2u * j, idesc, j > 0 ? 1u : (uint32_t)kb);
+                        else mma_bf16_ss(d, da + 2u * j, db + 2u * j, idesc, j > 0 ? 1u : (uint32_t)kb);
+                    }
+                    if (kPair) mma_commit_pair(&empty[s]);
+                    else mma_commit(&empty[s]);
+                    if (last) {
+                        if (kPair) mma_commit_pair(&acc_full[b]);
+                        else mma_commit(&acc_full[b]);
+                    }
                 }
-                if (kPair) mma_commit_pair(&empty[s]);
-                else mma_commit(&empty[s]);
+                __syncwarp();
                 issued = true;
-                if (++s == (uint32_t)kStages) {
-                    s = 0;
-                    phase ^= 1u;
+                ++kb;
+                if (last) {
+                    kb = 0;
+                    ++it;
+                    v += a.parts;
+                    stop = v >= tiles;
                 }
             }
-            if (stop) break;
-            if (kPair) mma_commit_pair(&acc_full[b]);
-            else mma_commit(&acc_full[b]);
+            phase ^= 1u;
         }
-        if (*abort && issued) {
-            if (kPair) mma_commit_pair_local(drain);
-            else mma_commit(drain);
+        if (aborted(abort) && issued) {
+            if (elect_lane()) {
+                if (kPair) mma_commit_pair_local(drain);
+                else mma_commit(drain);
+            }
+            __syncwarp();
             mbar_wait(drain, 0);
         }
     } else if (warp >= 2) {
@@ -609,7 +642,7 @@ struct FinishArgs {
     float *logprob, *entropy;
     int32_t *top_ids;
     float *top_logprobs;
-    int *redo;                         // [0] count, then (row, bits of m, bits of lse - m)
+    int *redo;                         // [0] count, counters of exact_kernel, (row, bits of m, bits of lse - m) ..
 };
 
 __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
@@ -626,6 +659,8 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
     const float4 *stats = p.stats + (size_t)block * nlists * kM + lrow;
     const uint2 *lists = p.lists + (size_t)block * nlists * kSlots * kM + lrow;
     stage_row(p.x + (size_t)row * p.H, p.H, xs);
+    pdl_launch_dependents();
+    pdl_wait();                                                     // score_kernel's lists and statistics
     if (tid == 0) {
         ncand = 0;
         tau_s = -INFINITY;
@@ -796,38 +831,47 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
     }
     if (!settled && lane == 0) {
         const int at = atomicAdd(p.redo, 1);
-        p.redo[1 + 3 * at] = row;
-        p.redo[2 + 3 * at] = __float_as_int(sum.m);
-        p.redo[3 + 3 * at] = __float_as_int(rest);
+        int *r = p.redo + 1 + kMaxClusters + 3 * at;
+        r[0] = row;
+        r[1] = __float_as_int(sum.m);
+        r[2] = __float_as_int(rest);
     }
 }
 
 // ------------------------------------------------------------------ rows the candidates do not settle
 
-constexpr int kExThreads = 512, kExWarps = kExThreads / 32, kExCluster = 8;
+constexpr int kExThreads = 512, kExWarps = kExThreads / 32;
 
 struct ExactArgs {
     const uint16_t *head, *x;
     int V, H, n;
-    const int *redo;
+    int *redo;
+    unsigned long long *lists;         // [clusters][32]
     int32_t *top_ids;
     float *top_logprobs;
 };
 
-// a cluster of kExCluster CTAs per row: every warp keeps the best of its vocabulary entries
+// Clusters of kExCluster CTAs take the rows in turn; fewer rows than clusters are split, each cluster
+// taking a share of the vocabulary, and the one that ends last joins the shares' lists.
 __global__ void __cluster_dims__(kExCluster, 1, 1) __launch_bounds__(kExThreads) exact_kernel(ExactArgs p) {
     extern __shared__ float xs[];
     __shared__ unsigned long long lists[kExWarps][32], gathered[kExCluster][32];
+    pdl_wait();
+    const int rows = *p.redo;
+    if (rows == 0) return;                                          // the same for every CTA
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int rows = *p.redo, clusters = gridDim.x / kExCluster;
-    if (rows == 0) return;                                          // the same for every CTA
-    for (int i = blockIdx.x / kExCluster; i < rows; i += clusters) {
-        const int row = p.redo[1 + 3 * i];
+    const int clusters = gridDim.x / kExCluster, me = blockIdx.x / kExCluster;
+    const int shares = rows < clusters ? clusters / rows : 1;
+    for (int unit = me; unit < rows * shares; unit += clusters) {
+        const int i = unit / shares, share = unit % shares;
+        const int *r = p.redo + 1 + kMaxClusters + 3 * i;
+        const int row = r[0];
         stage_row(p.x + (size_t)row * p.H, p.H, xs);
         __syncthreads();
         unsigned long long list = 0ull;
-        for (int v = rank * kExWarps + warp; v < p.V; v += kExCluster * kExWarps) {
+        const int step = shares * kExCluster * kExWarps;
+        for (int v = (share * kExCluster + rank) * kExWarps + warp; v < p.V; v += step) {
             const unsigned long long k = top_key(exact_logit(p.head + (size_t)v * p.H, xs, p.H), v);
             list = top_insert(list, k, 1u);
         }
@@ -844,9 +888,23 @@ __global__ void __cluster_dims__(kExCluster, 1, 1) __launch_bounds__(kExThreads)
         if (warp == 0) cluster.map_shared_rank(&gathered[0][0], 0)[rank * 32 + lane] = list;
         cluster.sync();
         if (rank == 0 && warp == 0) {
-            for (int r = 1; r < kExCluster; ++r) list = top_merge(list, gathered[r][lane]);
-            if (lane < p.n) {
-                const float m = __int_as_float(p.redo[2 + 3 * i]), rest = __int_as_float(p.redo[3 + 3 * i]);
+            for (int q = 1; q < kExCluster; ++q) list = top_merge(list, gathered[q][lane]);
+            bool mine = true;
+            if (shares > 1) {
+                p.lists[me * 32 + lane] = list;
+                __threadfence();
+                __syncwarp();
+                int before = 0;
+                if (lane == 0) before = atomicAdd(p.redo + 1 + i, 1);
+                before = __shfl_sync(0xffffffffu, before, 0);
+                __threadfence();
+                mine = before == shares - 1;
+                if (mine)
+                    for (int q = 0; q < shares; ++q)
+                        if (q != share) list = top_merge(list, __ldcg(p.lists + (i * shares + q) * 32 + lane));
+            }
+            if (mine && lane < p.n) {
+                const float m = __int_as_float(r[1]), rest = __int_as_float(r[2]);
                 p.top_ids[(size_t)row * p.n + lane] = top_index(list);
                 p.top_logprobs[(size_t)row * p.n + lane] = (top_value(list) - m) - rest;
             }
@@ -858,7 +916,7 @@ __global__ void __cluster_dims__(kExCluster, 1, 1) __launch_bounds__(kExThreads)
 struct Plan {
     int sms;
     bool paired;                       // 256-row blocks by CTA pairs, or one of 128 rows
-    size_t lists, stats, bins, redo, bytes;    // offsets
+    size_t lists, stats, bins, exact, redo, bytes;     // offsets
 };
 
 int make_plan(int T, Plan &pl) {
@@ -876,8 +934,9 @@ int make_plan(int T, Plan &pl) {
     pl.lists = 0;
     pl.stats = al256(slices * kSlots * kM * sizeof(uint2));
     pl.bins = pl.stats + al256(slices * kM * sizeof(float4));
-    pl.redo = pl.bins + al256(mblocks * kBins * kM * sizeof(unsigned));
-    pl.bytes = pl.redo + al256((1 + 3 * (size_t)rows) * sizeof(int));
+    pl.exact = pl.bins + al256(mblocks * kBins * kM * sizeof(unsigned));
+    pl.redo = pl.exact + al256((size_t)kMaxClusters * 32 * sizeof(unsigned long long));
+    pl.bytes = pl.redo + al256((1 + kMaxClusters + 3 * (size_t)rows) * sizeof(int));
     return MOE_OK;
 }
 
@@ -963,12 +1022,14 @@ extern "C" int moe_head_logprobs(const void *head, int V, int H, const void *x, 
         const FinishArgs fa{static_cast<const uint16_t *>(head), xr, V, H, n, parts, n + kPad, lists, stats,
                             targets ? targets + t0 : nullptr, logprob ? logprob + t0 : nullptr, entropy + t0, ids, tl,
                             redo};
-        finish_kernel<<<rows, kFinThreads, (size_t)H * sizeof(float), st>>>(fa);
-        MOE_CUDA_TRY(cudaGetLastError());
+        // both launched ahead of their predecessor's end (what they read of it they wait for)
+        MOE_CUDA_TRY(launch_pdl(finish_kernel, dim3((unsigned)rows), dim3(kFinThreads), (size_t)H * sizeof(float), st, fa));
         if (n > 0) {
-            const ExactArgs ea{static_cast<const uint16_t *>(head), xr, V, H, n, redo, ids, tl};
-            exact_kernel<<<(pl.sms / kExCluster) * kExCluster, kExThreads, (size_t)H * sizeof(float), st>>>(ea);
-            MOE_CUDA_TRY(cudaGetLastError());
+            const int clusters = pl.sms / kExCluster < kMaxClusters ? pl.sms / kExCluster : kMaxClusters;
+            const ExactArgs ea{static_cast<const uint16_t *>(head), xr, V, H, n, redo,
+                               reinterpret_cast<unsigned long long *>(ws + pl.exact), ids, tl};
+            MOE_CUDA_TRY(launch_pdl(exact_kernel, dim3((unsigned)(clusters * kExCluster)), dim3(kExThreads),
+                                    (size_t)H * sizeof(float), st, ea));
         }
     }
     return MOE_OK;

@@ -59,8 +59,10 @@ MOE_D bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort) {
     return ok;
 }
 
-// The same for one thread alone (a producer or issuer that its warp does not wait with).
-MOE_D bool wait_or_abort_thread(uint64_t *bar, uint32_t parity, volatile int *abort) {
+// The same without the vote, for a warp whose lanes all poll one barrier in step (the lanes see the same
+// phase): a few instructions when the barrier is ready.
+MOE_D bool wait_or_abort_step(uint64_t *bar, uint32_t parity, volatile int *abort) {
+    if (mbar_try_wait(bar, parity)) return true;
 #pragma unroll 1
     for (uint32_t i = 0; i < kMbarSpinLimit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -69,6 +71,13 @@ MOE_D bool wait_or_abort_thread(uint64_t *bar, uint32_t parity, volatile int *ab
     atomicOr(&g_moe_device_error, MOE_DEVERR_MBAR_TIMEOUT);
     *abort = 1;
     return false;
+}
+
+// true in one lane of the (converged) warp
+MOE_D bool elect_lane() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 
 MOE_D bool aborted(volatile int *abort) { return __any_sync(0xffffffffu, *abort != 0); }

@@ -322,11 +322,12 @@ def test_head_ties_and_padding_rows(dev):
     check_head(w, x, tg, 32)
 
 
-def test_head_near_ties(dev):
+@pytest.mark.parametrize("T", [1, 2, 9, 40, 150])
+def test_head_near_ties(dev, T):
     """Logits closer together than fp32 sums tell apart: the order is that of the 64-bit sums."""
     g = torch.Generator(device=dev)
     g.manual_seed(12)
-    H, V, T = 2048, 2000, 9
+    H, V = 2048, 2000
     base = torch.randn((1, H), generator=g, device=dev)
     w = (base * 0.02).to(torch.bfloat16).repeat(V, 1)
     # each row differs from the others in the last bit of a few of its smallest entries
