@@ -592,35 +592,37 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------ exact logits
 
-// x as floats, k-major (xs[k][c] = x[8 c + k]): lane-consecutive chunks read consecutive words
-MOE_D void stage_row(const uint16_t *x, int H, float *xs) {
+// x as floats: the elements 8 c .. 8 c + 3 of every chunk c of 8, then the elements 8 c + 4 .. 8 c + 7, so
+// that a warp's 16-byte reads of consecutive chunks do not meet in a bank
+MOE_D void stage_row(const uint16_t *x, int H, float4 *xs) {
     const int nch = H / 8;
     for (int c = threadIdx.x; c < nch; c += blockDim.x) {
         const uint4 q = __ldg(reinterpret_cast<const uint4 *>(x) + c);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            xs[(2 * k) * nch + c] = __uint_as_float(w[k] << 16);
-            xs[(2 * k + 1) * nch + c] = __uint_as_float(w[k] & 0xffff0000u);
-        }
+        xs[c] = make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16),
+                            __uint_as_float(q.y & 0xffff0000u));
+        xs[nch + c] = make_float4(__uint_as_float(q.z << 16), __uint_as_float(q.z & 0xffff0000u),
+                                  __uint_as_float(q.w << 16), __uint_as_float(q.w & 0xffff0000u));
     }
 }
 
 // A warp's dot product of a head row with the staged row: the products (exact in fp32) summed in
 // 64 bits in the LM head's order, rounded once
-MOE_D float exact_logit(const uint16_t *w, const float *xs, int H) {
+MOE_D float exact_logit(const uint16_t *w, const float4 *xs, int H) {
     const int lane = threadIdx.x & 31, nch = H / 8;
     const uint4 *wr = reinterpret_cast<const uint4 *>(w);
     double acc = 0.0;
 #pragma unroll 4
     for (int c = lane; c < nch; c += 32) {
         const uint4 q = __ldg(wr + c);
-        const uint32_t wv[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            acc += (double)(__uint_as_float(wv[j] << 16) * xs[(2 * j) * nch + c]);
-            acc += (double)(__uint_as_float(wv[j] & 0xffff0000u) * xs[(2 * j + 1) * nch + c]);
-        }
+        const float4 a = xs[c], b = xs[nch + c];
+        acc += (double)(__uint_as_float(q.x << 16) * a.x);
+        acc += (double)(__uint_as_float(q.x & 0xffff0000u) * a.y);
+        acc += (double)(__uint_as_float(q.y << 16) * a.z);
+        acc += (double)(__uint_as_float(q.y & 0xffff0000u) * a.w);
+        acc += (double)(__uint_as_float(q.z << 16) * b.x);
+        acc += (double)(__uint_as_float(q.z & 0xffff0000u) * b.y);
+        acc += (double)(__uint_as_float(q.w << 16) * b.z);
+        acc += (double)(__uint_as_float(q.w & 0xffff0000u) * b.w);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
@@ -629,8 +631,9 @@ MOE_D float exact_logit(const uint16_t *w, const float *xs, int H) {
 
 // ------------------------------------------------------------------ one row's parts joined
 
-constexpr int kFinThreads = 512, kFinWarps = kFinThreads / 32;
 constexpr int kCand = 1024;            // candidates that are ranked at once
+constexpr int kMaxLists = 512;         // lists of a row, at most
+constexpr int kGroups = 64;            // groups of threads whose maxima bound the candidates, with few lists
 
 struct FinishArgs {
     const uint16_t *head, *x;          // x: this launch's first row
@@ -645,12 +648,15 @@ struct FinishArgs {
     int *redo;                         // [0] count, counters of exact_kernel, (row, bits of m, bits of lse - m) ..
 };
 
-__global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
-    extern __shared__ float xs[];                                   // [H], k-major
+// kT: 512 threads for few rows (latency), 128 for many (the rows' own instructions are the bound then)
+template <int kT>
+__global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
+    constexpr int kW = kT / 32;
+    extern __shared__ float4 xs[];                                  // the row (stage_row)
     __shared__ unsigned long long cand[kCand], lead[kKeep];
-    __shared__ float peaks[kFinThreads], exact[kKeep + 1];
-    __shared__ int counts[kFinThreads];
-    __shared__ Soft softs[kFinWarps];
+    __shared__ float peaks[kMaxLists], exact[kKeep + 1];
+    __shared__ int counts[kMaxLists];
+    __shared__ Soft softs[kW];
     __shared__ float tau_s;
     __shared__ int ncand;
     const int row = blockIdx.x, block = row / kM, lrow = row % kM;
@@ -668,13 +674,11 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
 
     // statistics, in a fixed order
     Soft st = soft_none();
-    for (int l = tid; l < nlists; l += kFinThreads) {
+    for (int l = tid; l < nlists; l += kT) {
         const float4 f = stats[(size_t)l * kM];
         st = soft_merge(st, Soft{f.x, f.y, f.z});
-        if (l < kFinThreads) {
-            peaks[l] = f.x;
-            counts[l] = min(max(__float_as_int(f.w), 0), kSlots);
-        }
+        peaks[l] = f.x;
+        counts[l] = min(max(__float_as_int(f.w), 0), kSlots);
     }
     st = soft_warp(st);
     if (lane == 0) softs[warp] = st;
@@ -682,10 +686,10 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
 
     // the leading candidates: the keep-th largest of many disjoint maxima is a bound that keep entries
     // reach. With enough lists their own maxima do, and only the lists that reach the bound are read;
-    // else those of 64 groups of 8 threads, which hold the entries of 2 lists a warp
+    // else those of kGroups groups of threads, which hold the entries of 2 lists a warp
     constexpr int kPer = kSlots / 32;
-    const bool by_list = nlists >= 2 * p.keep && nlists <= kFinThreads;
-    const int npeaks = by_list ? nlists : kFinThreads / 8;
+    const bool by_list = nlists >= 2 * p.keep;
+    const int npeaks = by_list ? nlists : kGroups;
     uint2 held[2][kPer];
     auto load_list = [&](int l, uint2 (&e)[kPer]) {
 #pragma unroll
@@ -695,37 +699,37 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
     };
     if (!by_list) {
         float top = -INFINITY;
-        for (int l = warp; l < nlists; l += 2 * kFinWarps) {
+        for (int l = warp; l < nlists; l += 2 * kW) {
             load_list(l, held[0]);
-            load_list(l + kFinWarps, held[1]);
+            load_list(l + kW, held[1]);
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
                 top = fmaxf(top, fmaxf(__uint_as_float(held[0][i].x), __uint_as_float(held[1][i].x)));
         }
 #pragma unroll
-        for (int off = 4; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        for (int off = kT / kGroups / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         __syncthreads();                                            // (the lists' maxima are no longer needed)
-        if ((lane & 7) == 0) peaks[tid >> 3] = top;
+        if (tid % (kT / kGroups) == 0) peaks[tid / (kT / kGroups)] = top;
         __syncthreads();
     }
-    if (tid < npeaks) {
-        const float mine = peaks[tid];
+    for (int i = tid; i < npeaks; i += kT) {
+        const float mine = peaks[i];
         int r = 0;
 #pragma unroll 8
-        for (int j = 0; j < npeaks; ++j) r += (peaks[j] > mine || (peaks[j] == mine && j < tid)) ? 1 : 0;
+        for (int j = 0; j < npeaks; ++j) r += (peaks[j] > mine || (peaks[j] == mine && j < i)) ? 1 : 0;
         if (r == p.keep - 1) tau_s = mine;
     }
-    st = soft_warp(lane < kFinWarps ? softs[lane] : soft_none());
+    st = soft_warp(lane < kW ? softs[lane] : soft_none());
     __syncthreads();
     const float tau = tau_s;
-    const bool one_round = nlists <= 2 * kFinWarps;                  // held still has all entries
-    for (int l = warp; l < nlists; l += 2 * kFinWarps) {
+    const bool one_round = nlists <= 2 * kW;                  // held still has all entries
+    for (int l = warp; l < nlists; l += 2 * kW) {
         if (by_list || !one_round) {
             const bool a = !by_list || peaks[l] >= tau;
-            const bool b = l + kFinWarps < nlists && (!by_list || peaks[l + kFinWarps] >= tau);
+            const bool b = l + kW < nlists && (!by_list || peaks[l + kW] >= tau);
             if (!a && !b) continue;
             load_list(a ? l : nlists, held[0]);
-            load_list(b ? l + kFinWarps : nlists, held[1]);
+            load_list(b ? l + kW : nlists, held[1]);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -740,7 +744,7 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
     }
     __syncthreads();
     const int all = ncand, have = min(all, kCand);
-    for (int i = tid; i < have; i += kFinThreads) {
+    for (int i = tid; i < have; i += kT) {
         const unsigned long long k = cand[i];
         int r = 0;
         for (int j = 0; j < have; ++j) r += cand[j] > k ? 1 : 0;
@@ -752,7 +756,7 @@ __global__ void __launch_bounds__(kFinThreads) finish_kernel(FinishArgs p) {
     const int lead_n = min(have, p.keep);
     const int target = p.targets ? p.targets[row] : -1;
     const bool has_target = target >= 0 && target < p.V;
-    for (int i = warp; i <= lead_n; i += kFinWarps) {
+    for (int i = warp; i <= lead_n; i += kW) {
         const int id = i < lead_n ? top_index(lead[i]) : target;
         const bool in = id >= 0 && id < p.V;
         const float l = in ? exact_logit(p.head + (size_t)id * p.H, xs, p.H) : 0.f;
@@ -854,7 +858,7 @@ struct ExactArgs {
 // Clusters of kExCluster CTAs take the rows in turn; fewer rows than clusters are split, each cluster
 // taking a share of the vocabulary, and the one that ends last joins the shares' lists.
 __global__ void __cluster_dims__(kExCluster, 1, 1) __launch_bounds__(kExThreads) exact_kernel(ExactArgs p) {
-    extern __shared__ float xs[];
+    extern __shared__ float4 xs[];
     __shared__ unsigned long long lists[kExWarps][32], gathered[kExCluster][32];
     pdl_wait();
     const int rows = *p.redo;
@@ -923,9 +927,9 @@ int make_plan(int T, Plan &pl) {
     int dev = 0;
     MOE_CUDA_TRY(cudaGetDevice(&dev));
     MOE_CUDA_TRY(cudaDeviceGetAttribute(&pl.sms, cudaDevAttrMultiProcessorCount, dev));
-    if (pl.sms < 2 * kMaxGroup || pl.sms * kHalves > kFinThreads)
+    if (pl.sms < 2 * kMaxGroup || pl.sms * kHalves > kMaxLists)
         return moe_set_error(MOE_ENODEV, "head logprobs: a device of %d SMs (%d to %d)", pl.sms, 2 * kMaxGroup,
-                             kFinThreads / kHalves);
+                             kMaxLists / kHalves);
     pl.paired = T > kM;
     // 128-row blocks x parts is at most the number of SMs in every launch
     const size_t slices = (size_t)pl.sms * kHalves;
@@ -1023,13 +1027,17 @@ extern "C" int moe_head_logprobs(const void *head, int V, int H, const void *x, 
                             targets ? targets + t0 : nullptr, logprob ? logprob + t0 : nullptr, entropy + t0, ids, tl,
                             redo};
         // both launched ahead of their predecessor's end (what they read of it they wait for)
-        MOE_CUDA_TRY(launch_pdl(finish_kernel, dim3((unsigned)rows), dim3(kFinThreads), (size_t)H * sizeof(float), st, fa));
+        const size_t xbytes = (size_t)H * sizeof(float);
+        if (rows > 2 * pl.sms)
+            MOE_CUDA_TRY(launch_pdl(finish_kernel<128>, dim3((unsigned)rows), dim3(128), xbytes, st, fa));
+        else
+            MOE_CUDA_TRY(launch_pdl(finish_kernel<512>, dim3((unsigned)rows), dim3(512), xbytes, st, fa));
         if (n > 0) {
             const int clusters = pl.sms / kExCluster < kMaxClusters ? pl.sms / kExCluster : kMaxClusters;
             const ExactArgs ea{static_cast<const uint16_t *>(head), xr, V, H, n, redo,
                                reinterpret_cast<unsigned long long *>(ws + pl.exact), ids, tl};
             MOE_CUDA_TRY(launch_pdl(exact_kernel, dim3((unsigned)(clusters * kExCluster)), dim3(kExThreads),
-                                    (size_t)H * sizeof(float), st, ea));
+                                    xbytes, st, ea));
         }
     }
     return MOE_OK;
