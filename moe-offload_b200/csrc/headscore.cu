@@ -219,8 +219,8 @@ __device__ __noinline__ float list_cut(uint2 *list, int &count, int keep, int sp
 
 // A row's statistics while its tiles go by, in steps of 2: sums over 2^(x log2(e) - r) with r a whole
 // number near log2(e) times the largest value m, which the sums leave out (as SoftRun does). r is exact,
-// rescaling by it too, and one FMA makes an exponent. The constant's own rounding moves e^x by |x| 2^-24,
-// alike for values alike, and so do its uses here: fine for logits up to some hundreds.
+// rescaling by it too, and one FMA makes an exponent. The fp32 constant is 1.3e-8 off, which moves the
+// sums by 1.3e-8 |m| relative to e^m: 1e-5 at a logit of 1,000.
 struct Run2 {
     float m, r, s, w;                  // w: sum of t 2^t, t the exponents
 };

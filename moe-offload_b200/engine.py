@@ -26,10 +26,12 @@ from typing import Any
 import torch
 
 from . import checkpoint
+from .adapters import AdapterBank
 from .offload import HostExpertPool, OffloadStack, compute_layer_capacities
 from .synthetic import C2, StackConfig, dev_bf16_normal, dev_stack
 from .tokens import ByteTokenizer, TokenHead
 from .tokens import generate_stream as _generate_stream
+from .tokens import score_prompt as _score_prompt
 
 
 class OffloadEngine:
@@ -82,6 +84,8 @@ class OffloadEngine:
         if vocab_size is not None:
             self.token_head = TokenHead.synthetic(vocab_size, config.hidden, self.device, seed=config.seed + 101)
             self.tokenizer = ByteTokenizer(vocab_size)
+        self.adapters: AdapterBank | None = None
+        self.adapter_names: list[str] = []
         self._last_timings: dict[str, Any] = {}
         torch.cuda.synchronize(self.device)
         self.load_seconds = time.perf_counter() - t0
@@ -96,6 +100,19 @@ class OffloadEngine:
         if cap is not None:
             self.prefetch_cap = cap
             self.stack.prefetch_cap = cap
+
+    def set_adapters(self, bank: AdapterBank | None, names: list[str] | None = None) -> None:
+        """Low-rank adapters on the LM head (K = hidden, N = vocabulary) that generations choose by index or
+        name; None takes them away."""
+        if bank is not None:
+            if self.token_head is None:
+                raise RuntimeError("this engine has no token head: construct it with vocab_size=...")
+            if (bank.K, bank.N) != (self.token_head.H, self.token_head.V):
+                raise ValueError(f"adapters of {bank.K} x {bank.N} on a head of {self.token_head.H} x {self.token_head.V}")
+        names = [f"adapter-{i}" for i in range(bank.adapters if bank is not None else 0)] if names is None else list(names)
+        if len(names) != (0 if bank is None else bank.adapters) or len(set(names)) != len(names):
+            raise ValueError("one name of its own for each adapter expected")
+        self.adapters, self.adapter_names = bank, names
 
     def reset_caches(self) -> None:
         self.stack.reset_caches()
@@ -115,16 +132,42 @@ class OffloadEngine:
 
     # ------------------------------------------------------------------ generation
     def generate_stream(self, prompt_ids: list[int], max_tokens: int, temperature: float = 0.0, top_p: float = 1.0,
-                        stop_ids=None, seed: int = 0):
+                        stop_ids=None, seed: int = 0, adapter: int | str | None = None, logprobs: int | None = None,
+                        scored: list | None = None, prompt_scored: list | None = None):
         """server.py:113-199 `_generate_stream_impl`: token ids of the continuation of prompt_ids,
         one per decode step (greedy when temperature <= 0, else sampled with top_p), stopping at
-        the tokenizer's eos id, any of stop_ids, or max_tokens. Timings land in _last_timings."""
+        the tokenizer's eos id, any of stop_ids, or max_tokens. Timings land in _last_timings.
+        adapter: one of set_adapters', by index or name; logprobs, scored, prompt_scored: see
+        tokens.generate_stream."""
         if self.token_head is None:
             raise RuntimeError("this engine has no token head: construct it with vocab_size=...")
+        if isinstance(adapter, str):
+            if adapter not in self.adapter_names:
+                raise ValueError(f"no adapter is called {adapter!r}")
+            adapter = self.adapter_names.index(adapter)
         stops = {self.tokenizer.eos_token_id} | (set(int(x) for x in stop_ids) if stop_ids is not None else set())
         self._last_timings = {}
         return _generate_stream(self.stack, self.token_head, list(prompt_ids), max_tokens, temperature, top_p,
-                                stops, seed, self._last_timings)
+                                stops, seed, self._last_timings, self.adapters, -1 if adapter is None else int(adapter),
+                                logprobs, scored, prompt_scored)
+
+    def score_prompt(self, prompt_ids: list[int], n: int = 0, adapter: int | str | None = None) -> list[dict[str, Any]]:
+        """The log-probability, entropy and n most likely alternatives of each of prompt_ids[1:] given the ids
+        before it (one prefill): records as tokens.score_prompt returns them."""
+        if self.token_head is None:
+            raise RuntimeError("this engine has no token head: construct it with vocab_size=...")
+        if not prompt_ids:
+            raise ValueError("empty prompt")
+        if isinstance(adapter, str):
+            if adapter not in self.adapter_names:
+                raise ValueError(f"no adapter is called {adapter!r}")
+            adapter = self.adapter_names.index(adapter)
+        k = -1 if adapter is None else int(adapter)
+        if not -1 <= k < (0 if self.adapters is None else self.adapters.adapters):
+            raise ValueError(f"there is no adapter {k}")
+        ids = torch.tensor(list(prompt_ids), dtype=torch.int32).to(self.device)
+        rows = self.stack.prefill(self.token_head.embed(ids))
+        return _score_prompt(self.token_head, rows, list(prompt_ids), n, self.adapters, k)
 
     def generate_greedy(self, user_content: str = "", max_new_tokens: int = 128, reset_cache_before: bool = False,
                         reset_stats_before: bool = False, *, prompt_tokens: int | None = None) -> dict[str, Any]:

@@ -5,7 +5,9 @@ server.py:202-254).
 Kept: GET /v1/models, /health, /api/status (the engine's decode cache totals); POST
 /v1/completions and /v1/chat/completions with max_tokens / max_completion_tokens,
 temperature, top_p, seed, stop strings and `stream` (server-sent events, optional usage
-chunk); 400 for malformed requests, 404 for unknown paths; every generation on one worker
+chunk); `logprobs` (a number of alternatives for completions, with `echo` the prompt's own tokens
+too; `logprobs` / `top_logprobs` for chats) and, as `model`, the name of one of the engine's
+adapters; 400 for malformed requests, 404 for unknown paths; every generation on one worker
 thread, one request at a time. Left out (not on the MoE path): the Responses API, tool calls,
 thinking splits, the prompt cache, the web UI and the chat template of a real tokenizer (a chat
 prompt here is "role: content" lines and "assistant: ", encoded by the engine's tokenizer).
@@ -16,6 +18,7 @@ from __future__ import annotations
 
 import argparse
 import json
+import math
 import queue
 import threading
 import time
@@ -108,6 +111,57 @@ def _stop_strings(raw) -> list[str]:
     raise ValueError("'stop' must be a string or a list of strings")
 
 
+MAX_LOGPROBS = 20
+
+
+def _requested_logprobs(req: dict, is_chat: bool) -> int | None:
+    """The number of alternatives asked for with the tokens' log-probabilities; None for none at all."""
+    def count(key):
+        v = req.get(key)
+        if isinstance(v, bool) or not isinstance(v, int) or not 0 <= v <= MAX_LOGPROBS:
+            raise ValueError(f"'{key}' must be an integer from 0 to {MAX_LOGPROBS}")
+        return v
+    if not is_chat:
+        return None if req.get("logprobs") is None else count("logprobs")
+    if not isinstance(req.get("logprobs") or False, bool):
+        raise ValueError("'logprobs' must be true or false")
+    if req.get("top_logprobs") is not None and not req.get("logprobs"):
+        raise ValueError("'top_logprobs' needs 'logprobs'")
+    return (0 if req.get("top_logprobs") is None else count("top_logprobs")) if req.get("logprobs") else None
+
+
+def _finite(v: float) -> float | None:
+    return v if math.isfinite(v) else None           # (JSON has no infinities)
+
+
+def _token_text(tok, i: int) -> str:
+    """A token's text; ids that are no text of their own by number."""
+    text = tok.decode([i])
+    return text if text and "\ufffd" not in text else f"token_id:{i}"
+
+
+def _logprobs_json(tok, records: list[dict], is_chat: bool, offset: int = 0, first: bool = False) -> dict:
+    """The records of consecutive tokens in the response's form. Completions: offset is the first one's place in
+    the text, first: a prompt's first token stands before them, without a log-probability."""
+    if is_chat:
+        def entry(i, lp):
+            text = _token_text(tok, i)
+            return {"token": text, "logprob": _finite(lp), "bytes": list(text.encode())}
+        return {"content": [{**entry(r["id"], r["logprob"]), "top_logprobs": [entry(*t) for t in r["top"]]}
+                            for r in records]}
+    tokens = [_token_text(tok, r["id"]) for r in records]
+    offsets = []
+    for r in records:
+        offsets.append(offset)
+        offset += len(tok.decode([r["id"]]))
+    out = {"tokens": tokens, "token_logprobs": [_finite(r["logprob"]) for r in records],
+           "top_logprobs": [{_token_text(tok, i): _finite(lp) for i, lp in r["top"]} for r in records],
+           "text_offset": offsets}
+    if first:
+        out["token_logprobs"][0] = out["top_logprobs"][0] = None
+    return out
+
+
 def chat_prompt(messages) -> str:
     if not isinstance(messages, list) or not messages:
         raise ValueError("'messages' must be a non-empty list")
@@ -157,8 +211,10 @@ class Handler(BaseHTTPRequestHandler):
         if path in ("/health", "/healthz"):
             self._send_json(200, {"status": "ok", "model": srv.model_id, "busy": srv.worker.busy.locked()})
         elif path == "/v1/models":
-            self._send_json(200, {"object": "list", "data": [{"id": srv.model_id, "object": "model",
-                                                              "created": srv.created_ts, "owned_by": "local"}]})
+            names = [srv.model_id] + list(getattr(srv.engine, "adapter_names", []))
+            self._send_json(200, {"object": "list", "data": [{"id": name, "object": "model",
+                                                              "created": srv.created_ts, "owned_by": "local"}
+                                                             for name in names]})
         elif path == "/api/status":
             try:
                 lru, pref, dem, req, dem_b, pref_b = srv.engine._snapshot_decode_totals()
@@ -207,13 +263,18 @@ class Handler(BaseHTTPRequestHandler):
             seed = int(seed) if seed is not None else int(time.time_ns() & 0xFFFFFFFF)
             stops = _stop_strings(req.get("stop"))
             stream = bool(req.get("stream", False))
+            logprobs = _requested_logprobs(req, is_chat)
+            echo = bool(req.get("echo", False)) and not is_chat
+            names = getattr(srv.engine, "adapter_names", [])
+            adapter = req.get("model") if req.get("model") in names else None
             opts = req.get("stream_options") or {}
             include_usage = bool(isinstance(opts, dict) and opts.get("include_usage", False))
         except Exception as exc:  # noqa: BLE001
             self._send_error_json(400, str(exc), "invalid_request_error")
             return
         try:
-            self._generate(is_chat, prompt_ids, max_tokens, temperature, top_p, seed, stops, stream, include_usage)
+            self._generate(is_chat, prompt_ids, max_tokens, temperature, top_p, seed, stops, stream, include_usage,
+                           logprobs, echo, adapter)
         except Exception as exc:  # noqa: BLE001
             try:
                 self._send_error_json(500, str(exc), "server_error")
@@ -221,7 +282,7 @@ class Handler(BaseHTTPRequestHandler):
                 pass
 
     def _generate(self, is_chat, prompt_ids, max_tokens, temperature, top_p, seed, stops, stream,
-                  include_usage) -> None:
+                  include_usage, logprobs=None, echo=False, adapter=None) -> None:
         srv = self.server
         tok = srv.engine.tokenizer
         rid = ("chatcmpl-" if is_chat else "cmpl-") + uuid.uuid4().hex[:24]
@@ -231,8 +292,32 @@ class Handler(BaseHTTPRequestHandler):
         text, sent, finish = "", 0, "length"
         t0 = time.perf_counter()
         timings: dict = {}
+        # records of the generated tokens (and, with echo, of the prompt's): complete up to a token when it arrives
+        scored: list[dict] = []
+        prompt_scored: list[dict] = []
+        more = {}
+        if logprobs is not None:
+            more = {"logprobs": logprobs, "scored": scored, **({"prompt_scored": prompt_scored} if echo else {})}
+        if adapter is not None:
+            more["adapter"] = adapter
+        model = srv.model_id if adapter is None else adapter
+        head = tok.decode(prompt_ids) if echo else ""
         gen = srv.worker.stream(prompt_ids, max_tokens, temperature=temperature, top_p=top_p, seed=seed,
-                                timings=timings)
+                                timings=timings, **more)
+        told = 0
+
+        def lp_of(last: int):
+            """The response's logprobs of the tokens from `told` up to `last`, with the echoed prompt's before the
+            first."""
+            nonlocal told
+            if logprobs is None:
+                return None
+            part, at, first = scored[told:last], told, echo and told == 0 and bool(prompt_ids)
+            if first:
+                part = [{"id": prompt_ids[0], "logprob": math.nan, "top": []}] + prompt_scored + part
+            told = last
+            start = 0 if first else len(head) + len(tok.decode(ids[:at]))
+            return _logprobs_json(tok, part, is_chat, start, first)
         if stream:
             self.send_response(200)
             self.send_header("Content-Type", "text/event-stream")
@@ -240,7 +325,7 @@ class Handler(BaseHTTPRequestHandler):
             self.send_header("Transfer-Encoding", "chunked")
             self.end_headers()
             if is_chat:
-                self._sse(self._chunk(rid, created, is_chat, {"role": "assistant", "content": ""}, None))
+                self._sse(self._chunk(rid, created, is_chat, {"role": "assistant", "content": ""}, None, model))
         try:
             for t in gen:
                 ids.append(t)
@@ -249,7 +334,8 @@ class Handler(BaseHTTPRequestHandler):
                 if hit >= 0:
                     text, finish = text[:hit], "stop"
                 if stream and len(text) > sent and "�" not in text[sent:]:
-                    self._sse(self._chunk(rid, created, is_chat, text[sent:], None))
+                    piece = (head if sent == 0 else "") + text[sent:]
+                    self._sse(self._chunk(rid, created, is_chat, piece, None, model, lp_of(len(ids))))
                     sent = len(text)
                 if hit >= 0:
                     break
@@ -262,30 +348,34 @@ class Handler(BaseHTTPRequestHandler):
         srv.last_request = {"id": rid, "prompt_tokens": len(prompt_ids), "completion_tokens": len(ids),
                             "seconds": round(time.perf_counter() - t0, 4), "timings": timings}
         if stream:
-            if len(text) > sent:
-                self._sse(self._chunk(rid, created, is_chat, text[sent:], None))
-            self._sse(self._chunk(rid, created, is_chat, "" if not is_chat else {}, finish))
+            if len(text) > sent or (echo and sent == 0) or (logprobs is not None and told < len(ids)):
+                piece = (head if sent == 0 else "") + text[sent:]
+                self._sse(self._chunk(rid, created, is_chat, piece, None, model, lp_of(len(ids))))
+            self._sse(self._chunk(rid, created, is_chat, "" if not is_chat else {}, finish, model))
             if include_usage:
-                self._sse({"id": rid, "object": obj + ".chunk", "created": created, "model": srv.model_id,
+                self._sse({"id": rid, "object": obj + ".chunk", "created": created, "model": model,
                            "choices": [], "usage": usage})
             self._sse("[DONE]")
             self.wfile.write(b"0\r\n\r\n")
             self.wfile.flush()
             return
         choice = ({"index": 0, "message": {"role": "assistant", "content": text}, "finish_reason": finish}
-                  if is_chat else {"index": 0, "text": text, "finish_reason": finish})
-        self._send_json(200, {"id": rid, "object": obj, "created": created, "model": srv.model_id,
+                  if is_chat else {"index": 0, "text": head + text, "finish_reason": finish})
+        if logprobs is not None:
+            choice["logprobs"] = lp_of(len(ids))
+        self._send_json(200, {"id": rid, "object": obj, "created": created, "model": model,
                               "choices": [choice], "usage": usage})
 
-    def _chunk(self, rid, created, is_chat, delta, finish) -> dict:
-        srv = self.server
+    def _chunk(self, rid, created, is_chat, delta, finish, model, logprobs=None) -> dict:
         if is_chat:
             d = delta if isinstance(delta, dict) else {"content": delta}
             choice = {"index": 0, "delta": d, "finish_reason": finish}
-            return {"id": rid, "object": "chat.completion.chunk", "created": created, "model": srv.model_id,
-                    "choices": [choice]}
-        return {"id": rid, "object": "text_completion", "created": created, "model": srv.model_id,
-                "choices": [{"index": 0, "text": delta, "finish_reason": finish}]}
+        else:
+            choice = {"index": 0, "text": delta, "finish_reason": finish}
+        if logprobs is not None:
+            choice["logprobs"] = logprobs
+        return {"id": rid, "object": "chat.completion.chunk" if is_chat else "text_completion", "created": created,
+                "model": model, "choices": [choice]}
 
 
 def make_server(engine, host: str = "127.0.0.1", port: int = 8000, model_id: str = "moe-offload-b200",

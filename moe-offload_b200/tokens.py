@@ -141,14 +141,18 @@ class TokenHead:
              _stream(stream))
         return out
 
-    def logits(self, h: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
-        """h bf16 [T, H] (T <= 4) -> fp32 [T, V]."""
+    def logits(self, h: torch.Tensor, out: torch.Tensor | None = None, stream=None, adapters=None,
+               adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
+        """h bf16 [T, H] (T <= 4) -> fp32 [T, V]. adapters (adapters.AdapterBank of K = H, N = V) with
+        adapter_ids int32 [T] (device): each row's low-rank adapter is added, -1 for none."""
         _need(h, "h", (torch.bfloat16,), self.device)
         T = h.shape[0]
         if out is None:
             out = torch.empty((T, self.V), dtype=torch.float32, device=self.device)
         call("moe_lm_head_logits", self.head_w.data_ptr(), self.V, self.H, h.data_ptr(), T, out.data_ptr(),
              _stream(stream))
+        if adapters is not None:
+            adapters.add(out, h, adapter_ids, out=out, stream=stream)
         return out
 
     def argmax(self, h: torch.Tensor, out: torch.Tensor | None = None, logits: torch.Tensor | None = None,
@@ -188,15 +192,48 @@ class TokenHead:
         return out
 
 
+def _records(ids: list[int], r: TokenLogprobs) -> list[dict[str, Any]]:
+    """One host record per row: id, logprob, entropy, top [(id, logprob), ..] (a read of the device)."""
+    lp, ent = r.logprob.tolist(), r.entropy.tolist()
+    ti, tl = r.top_ids.tolist(), r.top_logprobs.tolist()
+    return [{"id": i, "logprob": lp[t], "entropy": ent[t], "top": list(zip(ti[t], tl[t]))} for t, i in enumerate(ids)]
+
+
+def score_prompt(head: TokenHead, rows: torch.Tensor, prompt_ids: list[int], n: int = 0, adapters=None,
+                 adapter: int = -1) -> list[dict[str, Any]]:
+    """Records of prompt_ids[1:], each under the row before it: rows bf16 [len(prompt_ids), H] are the stack's
+    outputs. With an adapter the logits come four rows at a time (TokenHead.logits); without one straight
+    from the rows (TokenHead.score)."""
+    if len(prompt_ids) < 2:
+        return []
+    ids = torch.tensor(list(prompt_ids[1:]), dtype=torch.int32).to(head.device, non_blocking=True)
+    if adapters is None or adapter < 0:
+        return _records(list(prompt_ids[1:]), head.score(rows[:-1].contiguous(), ids, n))
+    of = torch.full((4,), adapter, dtype=torch.int32, device=head.device)
+    out: list[dict[str, Any]] = []
+    for t in range(0, len(prompt_ids) - 1, 4):
+        m = min(4, len(prompt_ids) - 1 - t)
+        logits = head.logits(rows[t:t + m].contiguous(), adapters=adapters, adapter_ids=of[:m])
+        out += _records(list(prompt_ids[1 + t:1 + t + m]), token_logprobs(logits, ids[t:t + m], n))
+    return out
+
+
 def generate_stream(stack, head: TokenHead, prompt_ids: list[int], max_tokens: int, temperature: float = 0.0,
                     top_p: float = 1.0, stop_ids: Iterable[int] | None = None, seed: int = 0,
-                    timings: dict[str, Any] | None = None) -> Iterator[int]:
+                    timings: dict[str, Any] | None = None, adapters=None, adapter: int = -1,
+                    logprobs: int | None = None, scored: list | None = None,
+                    prompt_scored: list | None = None) -> Iterator[int]:
     """server.py:113-199 as a token-id generator over `stack` (anything with prefill(rows [T, H])
     -> [T, H] and decode_token(h [1, H]) -> [1, H], e.g. offload.OffloadStack): prefill of the
     prompt's embedding rows, the next id from the last row's logits, then one decode step per
     yielded id until max_tokens, a stop id, or the caller stops iterating. `timings` receives
     prefill_s, decode_s, decode_tok_per_s, stopped_by_token (the reference's keys). Each step
-    reads its id back to the host (the stop test), as the reference does."""
+    reads its id back to the host (the stop test), as the reference does.
+
+    adapters / adapter: a bank of low-rank adapters on the LM head and the one this generation uses
+    (-1: none). logprobs = n: `scored` receives a record of every yielded id before it is yielded (id,
+    logprob, entropy, top: the n most likely ids with their log-probabilities, of the distribution
+    before temperature and top_p), and `prompt_scored`, when given, those of prompt_ids[1:]."""
     stop_set = set(int(x) for x in stop_ids) if stop_ids is not None else set()
     tm = timings if timings is not None else {}
     tm.update({"prefill_s": 0.0, "decode_s": 0.0, "decode_tok_per_s": 0.0, "stopped_by_token": False})
@@ -204,15 +241,25 @@ def generate_stream(stack, head: TokenHead, prompt_ids: list[int], max_tokens: i
         return
     if not prompt_ids:
         raise ValueError("empty prompt")
+    if adapters is not None and not -1 <= adapter < adapters.adapters:
+        raise ValueError(f"adapter {adapter}: the bank has {adapters.adapters}")
+    if adapters is None and adapter >= 0:
+        raise ValueError(f"adapter {adapter}: there is no bank of adapters")
     dev = head.device
     t0 = time.perf_counter()
+    bank = adapters if adapter >= 0 else None
+    of = None if bank is None else torch.full((1,), adapter, dtype=torch.int32).to(dev)
     ids = torch.tensor(list(prompt_ids), dtype=torch.int32).to(dev, non_blocking=True)
     rows = head.embed(ids)
     out = stack.prefill(rows)
     greedy = not temperature > 0.0
-    logits = head.logits(out[-1:].contiguous())
+    # the fused head and argmax leave no logits to adapt or score
+    fused = greedy and bank is None and logprobs is None
+    logits = head.logits(out[-1:].contiguous(), adapters=bank, adapter_ids=of)
     cur = head.sample(logits, temperature, top_p, seed, 0)
     tok = int(cur.item())
+    if logprobs is not None and prompt_scored is not None:
+        prompt_scored += score_prompt(head, out, list(prompt_ids), logprobs, bank, adapter)
     tm["prefill_s"] = round(time.perf_counter() - t0, 4)
     n = 0
     t_dec0 = time.perf_counter()
@@ -222,14 +269,16 @@ def generate_stream(stack, head: TokenHead, prompt_ids: list[int], max_tokens: i
                 tm["stopped_by_token"] = True
                 break
             n += 1
+            if logprobs is not None and scored is not None:
+                scored += _records([tok], token_logprobs(logits, cur, logprobs))
             yield tok
             if d + 1 >= max_tokens:
                 break
             y = stack.decode_token(head.embed(cur))
-            if greedy:
+            if fused:
                 head.argmax(y, out=cur)
             else:
-                head.logits(y, out=logits)
+                head.logits(y, out=logits, adapters=bank, adapter_ids=of)
                 head.sample(logits, temperature, top_p, seed, d + 1, out=cur)
             tok = int(cur.item())
     finally:
