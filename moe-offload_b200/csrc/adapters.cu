@@ -15,8 +15,9 @@
 // straight from 16-byte global loads. For that the K order inside a step is permuted alike in both
 // operands: a lane's consecutive elements fill its places of the fragments.
 //
-// u is carried into the second product as two bf16 (u = hi + lo, off by 2^-17 of u at most): the fp32
-// logits of an adapted head must not lose digits that one bf16 would drop.
+// u is carried into the second product as a sum of bf16 numbers: two of them (off by 2^-17 of u at most)
+// for bf16 outputs, whose own rounding is 2^-8, and three, which hold all of an fp32 number's 24 bits, for
+// an adapted head's fp32 logits (with two these were 2e-6 off, with three 1e-7).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -63,14 +64,14 @@ MOE_D float below_bf16(float v) {
 }
 
 // kMT: row fragments (16 rows) a tile; kNT: fragments of 8 rank rows the warps have registers for
-template <int kMT, int kNT>
+template <int kMT, int kNT, int kParts>
 struct Smem {
     static constexpr int kRows = 16 * kMT, kWK = kWarps / kMT;       // warps along K per row fragment
     static constexpr int kR = 8 * kNT, kSteps = (kR + 15) / 16;
     static constexpr int kF = kNT == 2 ? 8 : 4;  // output fragments of 8 a warp takes at a time
     float part[kWK][kRows][kR];        // the warps' sums over their K steps
     float u[kRows][kR];                // the CTA's sums, read by the cluster
-    uint4 frag[2][kMT][kSteps][32];    // scale * u as fragments: high and low parts
+    uint4 frag[kParts][kMT][kSteps][32];         // scale * u as fragments: high to low parts
     int row[kRows], id[kRows];         // the tile's rows and their adapters
     int kind[kRows];                   // the different ones among them
     unsigned member[kRows];            // which rows are of that kind
@@ -220,7 +221,8 @@ MOE_D int tile_rows(S &sh, const AdapterArgs &p, int tile, bool report) {
 // two CTAs an SM where the registers allow it: the kernel is a chain of short dependent phases
 template <int kMT, int kNT, bool kFp32>
 __global__ void __launch_bounds__(kThreads, kNT <= 8 ? 2 : 1) adapter_kernel(AdapterArgs p) {
-    using S = Smem<kMT, kNT>;
+    constexpr int kParts = kFp32 ? 3 : 2;
+    using S = Smem<kMT, kNT, kParts>;
     extern __shared__ __align__(16) unsigned char smem[];
     S &sh = *reinterpret_cast<S *>(smem);
     cg::cluster_group cluster = cg::this_cluster();
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, kNT <= 8 ? 2 : 1) adapter_kernel(Ada
     for (int i = tid; i < kMT * S::kSteps * 32; i += kThreads) {
         const int l = i & 31, s = (i >> 5) % S::kSteps, m = (i >> 5) / S::kSteps;
         const int c = 16 * s + 4 * (l & 3);
-        uint32_t hi[4], lo[4];
+        uint32_t f[kParts][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int r = 16 * m + (l >> 2) + 8 * h;
@@ -313,16 +315,18 @@ __global__ void __launch_bounds__(kThreads, kNT <= 8 ? 2 : 1) adapter_kernel(Ada
                     const float4 o = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(&sh.u[r][c], k));
                     v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
                 }
-                const float f = __ldg(p.scale + sh.id[r]);
-                v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+                const float scale = __ldg(p.scale + sh.id[r]);
+                v.x *= scale; v.y *= scale; v.z *= scale; v.w *= scale;
             }
-            hi[h] = pack_bf16(v.x, v.y);
-            hi[2 + h] = pack_bf16(v.z, v.w);
-            lo[h] = pack_bf16(below_bf16(v.x), below_bf16(v.y));
-            lo[2 + h] = pack_bf16(below_bf16(v.z), below_bf16(v.w));
+#pragma unroll
+            for (int q3 = 0; q3 < kParts; ++q3) {
+                f[q3][h] = pack_bf16(v.x, v.y);
+                f[q3][2 + h] = pack_bf16(v.z, v.w);
+                v = make_float4(below_bf16(v.x), below_bf16(v.y), below_bf16(v.z), below_bf16(v.w));
+            }
         }
-        sh.frag[0][m][s][l] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        sh.frag[1][m][s][l] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+        for (int q3 = 0; q3 < kParts; ++q3) sh.frag[q3][m][s][l] = make_uint4(f[q3][0], f[q3][1], f[q3][2], f[q3][3]);
     }
     __syncthreads();
     if (ctas > 1) cluster.barrier_arrive();      // this CTA has read the others' u (waited for at the end)
@@ -377,11 +381,12 @@ __global__ void __launch_bounds__(kThreads, kNT <= 8 ? 2 : 1) adapter_kernel(Ada
 #pragma unroll
                     for (int m = 0; m < kMT; ++m) {
                         if (kMT > 1 && !(sh.member[d] & (0xffffu << (16 * m)))) continue;
-                        const uint4 hi = sh.frag[0][m][s0 + s][lane], lo = sh.frag[1][m][s0 + s][lane];
 #pragma unroll
-                        for (int f = 0; f < kF; ++f) mma16816(sum[m][f], hi.x, hi.y, hi.z, hi.w, w[s][f].x, w[s][f].y);
+                        for (int h = 0; h < kParts; ++h) {
+                            const uint4 u = sh.frag[h][m][s0 + s][lane];
 #pragma unroll
-                        for (int f = 0; f < kF; ++f) mma16816(sum[m][f], lo.x, lo.y, lo.z, lo.w, w[s][f].x, w[s][f].y);
+                            for (int f = 0; f < kF; ++f) mma16816(sum[m][f], u.x, u.y, u.z, u.w, w[s][f].x, w[s][f].y);
+                        }
                     }
                 }
             }
@@ -429,7 +434,7 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb) {
 template <int kMT, int kNT, bool kFp32>
 int launch(const AdapterArgs &p, int ctas, cudaStream_t st) {
     auto kern = adapter_kernel<kMT, kNT, kFp32>;
-    const size_t smem = sizeof(Smem<kMT, kNT>);
+    const size_t smem = sizeof(Smem<kMT, kNT, kFp32 ? 3 : 2>);
     MOE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((p.T + p.rows - 1) / p.rows) * (unsigned)p.splits * (unsigned)ctas);
