@@ -335,7 +335,7 @@ int moe_token_logprobs_launch(const float *logits, int T, int V, const int32_t *
     attr[0].val.clusterDim.x = (unsigned)parts;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = parts > 1 ? 1 : 0;            // (a CTA alone is a cluster of one)
     const LogprobArgs p{logits, T, V, n, targets, logprob, entropy, top_ids, top_logprobs};
     MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, logprobs_kernel, p));
     return MOE_OK;

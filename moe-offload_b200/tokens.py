@@ -34,17 +34,21 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor
 
 
-def _logprob_outputs(T: int, V: int, targets: torch.Tensor | None, n: int, dev) -> TokenLogprobs:
+def _logprob_outputs(like: torch.Tensor, T: int, V: int, targets: torch.Tensor | None, n: int) -> TokenLogprobs:
     if not 0 <= n <= min(V, MAX_ALTERNATIVES):
         raise ValueError(f"{n} alternatives: 0 to {min(V, MAX_ALTERNATIVES)} can be asked for")
     if targets is not None:
-        _need(targets, "targets", (torch.int32,), dev)
+        _need(targets, "targets", (torch.int32,), like.device)
         if targets.numel() != T:
             raise ValueError(f"{targets.numel()} targets for {T} rows")
-    return TokenLogprobs(None if targets is None else torch.empty((T,), dtype=torch.float32, device=dev),
-                         torch.empty((T,), dtype=torch.float32, device=dev),
-                         torch.empty((T, n), dtype=torch.int32, device=dev),
-                         torch.empty((T, n), dtype=torch.float32, device=dev))
+    # (new_empty: a third less host time than torch.empty, which parses a device)
+    f = torch.float32
+    if like.dtype != f:
+        return TokenLogprobs(None if targets is None else like.new_empty(T, dtype=f), like.new_empty(T, dtype=f),
+                             like.new_empty((T, n), dtype=torch.int32), like.new_empty((T, n), dtype=f))
+    return TokenLogprobs(None if targets is None else like.new_empty(T), like.new_empty(T),
+                         like.new_empty((T, n), dtype=torch.int32) if targets is None else targets.new_empty((T, n)),
+                         like.new_empty((T, n)))
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, n: int = 0,
@@ -57,7 +61,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, n:
     T, V = logits.shape
     dev = logits.device
     with _launch_on(dev, stream):
-        r = _logprob_outputs(T, V, targets, n, dev)
+        r = _logprob_outputs(logits, T, V, targets, n)
         if T:
             call("moe_token_logprobs", logits.data_ptr(), T, V, _ptr(targets), n, _ptr(r.logprob),
                  r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), _stream(stream, dev))
@@ -76,7 +80,7 @@ def head_logprobs(head: torch.Tensor, h: torch.Tensor, targets: torch.Tensor | N
     V, H = head.shape
     T = h.shape[0]
     with _launch_on(dev, stream):
-        r = _logprob_outputs(T, V, targets, n, dev)
+        r = _logprob_outputs(h, T, V, targets, n)
         if T:
             ws = torch.empty(int(call("moe_head_logprobs_workspace_bytes", T, V, n)), dtype=torch.uint8, device=dev)
             call("moe_head_logprobs", head.data_ptr(), V, H, h.data_ptr(), T, _ptr(targets), n, _ptr(r.logprob),
