@@ -41,7 +41,7 @@ constexpr int kHalves = 2;
 constexpr uint32_t kABytes = kM * 128;
 constexpr uint32_t kTmemCols = 512;    // two accumulators of kN columns: one fills while one is read
 
-constexpr int kSlots = 64;             // a row's list in one part
+constexpr int kSlots = 160;            // a row's list in one part: a first tile whole (128), and some
 constexpr int kPad = 8;                // kept beyond n, to tell whether the order of the n is settled
 constexpr int kKeep = kTopMax + kPad;  // at most
 constexpr int kBins = 64;              // disjoint maxima of a row, for a bound on its keep-th largest logit
@@ -122,9 +122,8 @@ MOE_D void arrive_first_cta(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// 32 columns of this warp's 32 TMEM lanes
-MOE_D void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
+// 32 columns of this warp's 32 TMEM lanes; r holds them after tmem_wait (nothing may touch it before)
+MOE_D void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
         "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -133,9 +132,16 @@ MOE_D void tmem_ld32(uint32_t taddr, float (&v)[32]) {
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+MOE_D void tmem_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
 }
 
 // order-preserving image of a float that is no NaN (-0 below +0: both forms of a zero logit are
@@ -151,72 +157,6 @@ MOE_D float value_of(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o
 // +0); -inf for none
 MOE_D float value_below(uint32_t o) { return o > 0x00800000u ? value_of(o - (o == 0x80000000u ? 2u : 1u)) : -INFINITY; }
 
-// Cuts a thread's list (more than keep + spare entries) down to its keep largest entries, or up to
-// spare more where that ends the search sooner. Equal entries that do not all fit stay lowest index
-// first (the list is in index order, and stays so). Returns a value that at least keep of the kept
-// entries reach: what comes later and does not exceed it is not among the keep largest. The 32 rows of
-// a warp work side by side, each bisecting for its own bound by counting.
-// (Not inlined: it is hardly ever called, and its registers would spill those of the common path.)
-__device__ __noinline__ float list_cut(uint2 *list, int &count, int keep, int spare) {
-    uint32_t o[kSlots];
-    uint32_t lo = 0xffffffffu, hi = 0u;
-    // (slots behind the list are read too, and left out)
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) o[i] = list[i * kM].x;
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) {
-        o[i] = i < count ? order_of(__uint_as_float(o[i])) : 0u;
-        hi = max(hi, o[i]);
-        lo = min(lo, o[i] - 1u);                  // (0 - 1: the largest)
-    }
-    // at least keep entries reach lo, fewer reach hi
-    int reach = count;
-    lo += 1u;
-    hi += 1u;
-#pragma unroll 1
-    while (reach > keep + spare && hi - lo > 1u) {
-        const uint32_t mid = lo + (hi - lo) / 2u;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) n += o[i] >= mid ? 1 : 0;
-        if (n >= keep) {
-            lo = mid;
-            reach = n;
-        } else {
-            hi = mid;
-        }
-    }
-    int ties = kSlots;                            // how many of those equal to lo stay
-    if (reach > keep + spare) {
-        ties = keep;
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i) ties -= o[i] > lo ? 1 : 0;
-    }
-    // 16 indices in flight while the 16 before are moved (down, so never onto those)
-    constexpr int kB = 16;
-    uint32_t id[2][kB];
-    int at = 0;
-#pragma unroll
-    for (int i = 0; i < kB; ++i) id[0][i] = list[i * kM].y;
-#pragma unroll
-    for (int i0 = 0; i0 < kSlots; i0 += kB) {
-        if (i0 + kB < kSlots) {
-#pragma unroll
-            for (int i = 0; i < kB; ++i) id[(i0 / kB + 1) & 1][i] = list[(i0 + kB + i) * kM].y;
-        }
-#pragma unroll
-        for (int i = 0; i < kB; ++i) {
-            const uint32_t k = o[i0 + i];
-            if (k > lo || (k == lo && ties-- > 0)) {
-                list[at * kM] = make_uint2(__float_as_uint(value_of(k)), id[(i0 / kB) & 1][i]);
-                ++at;
-            }
-        }
-    }
-    count = at;
-    return value_of(lo);
-}
-
 // A row's statistics while its tiles go by, in steps of 2: sums over 2^(x log2(e) - r) with r a whole
 // number near log2(e) times the largest value m, which the sums leave out (as SoftRun does). r is exact,
 // rescaling by it too, and one FMA makes an exponent. The fp32 constant is 1.3e-8 off, which moves the
@@ -224,9 +164,11 @@ __device__ __noinline__ float list_cut(uint2 *list, int &count, int keep, int sp
 struct Run2 {
     float m, r, s, w;                  // w: sum of t 2^t, t the exponents
 };
-// 32 values, top their largest (NaN left out)
-MOE_D void run2_add(Run2 &a, const float (&x)[32], float top) {
-    float s[2] = {a.s, 0.f}, w[2] = {a.w, 0.f};
+// 32 values, top their largest (NaN left out). Columns that are not there hold kAbsent, not -inf: 0 x inf
+// would be NaN.
+constexpr float kAbsent = -1e30f;
+MOE_D void run2_add(Run2 &a, const uint32_t (&x)[32], float top) {
+    float s[4] = {a.s, 0.f, 0.f, 0.f}, w[4] = {a.w, 0.f, 0.f, 0.f};
     if (__any_sync(0xffffffffu, top > a.m)) {     // somebody's largest value changes
         const float want = floorf(top * kLog2e);
         if (top > a.m && !(want <= a.r + 40.f && a.m > -INFINITY)) {
@@ -237,21 +179,22 @@ MOE_D void run2_add(Run2 &a, const float (&x)[32], float top) {
         }
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float t = fmaf(min_nan(a.m, x[i]), kLog2e, -a.r), e = fast_pow2(t);
-            a.m = fmaxf(a.m, x[i]);
-            s[i & 1] += e;
-            w[i & 1] = fmaf(fmaxf(t, kSoftFar), e, w[i & 1]);
+            const float v = __uint_as_float(x[i]);
+            const float t = fmaf(fmaxf(min_nan(a.m, v), kAbsent), kLog2e, -a.r), e = fast_pow2(t);
+            a.m = fmaxf(a.m, v);
+            s[i & 3] += fabsf(v) < INFINITY ? e : v - v;            // NaN for what is not finite
+            w[i & 3] = fmaf(t, e, w[i & 3]);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float t = fmaf(x[i], kLog2e, -a.r), e = fast_pow2(t);
-            s[i & 1] += e;
-            w[i & 1] = fmaf(fmaxf(t, kSoftFar), e, w[i & 1]);
+            const float t = fmaf(__uint_as_float(x[i]), kLog2e, -a.r), e = fast_pow2(t);
+            s[i & 3] += e;
+            w[i & 3] = fmaf(t, e, w[i & 3]);
         }
     }
-    a.s = s[0] + s[1];
-    a.w = w[0] + w[1];
+    a.s = (s[0] + s[1]) + (s[2] + s[3]);
+    a.w = (w[0] + w[1]) + (w[2] + w[3]);
 }
 
 MOE_D Soft run2_end(const Run2 &a) {
@@ -264,13 +207,20 @@ MOE_D Soft run2_end(const Run2 &a) {
 // A bound that at least keep of the row's logits reach, from its maxima so far in kBins disjoint sets
 // of vocabulary entries (kM apart): their keep-th largest, or a little less. 0: fewer maxima than that.
 MOE_D uint32_t bins_bound(const uint32_t (&o)[kBins], int keep) {
-    uint32_t lo = 0u, hi = 0u;
+    uint32_t lo = 0xffffffffu, hi = 0u;
+    int reach = 0;
 #pragma unroll
-    for (int i = 0; i < kBins; ++i) hi = max(hi, o[i]);
-    int reach = kBins;
+    for (int i = 0; i < kBins; ++i) {
+        hi = max(hi, o[i]);
+        lo = min(lo, o[i] - 1u);                  // (0 - 1: the largest)
+        reach += o[i] ? 1 : 0;
+    }
+    if (reach < keep) return 0u;
+    // reach >= keep bins reach lo, fewer reach hi
+    lo += 1u;
     hi += 1u;
 #pragma unroll 1
-    while (reach > keep + 6 && hi - lo > 1u) {
+    while (reach > keep + 4 && hi - lo > 1u) {
         const uint32_t mid = lo + (hi - lo) / 2u;
         int n = 0;
 #pragma unroll
@@ -467,103 +417,124 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint2 *list = a.lists + (size_t)slice * kSlots * kM + lrow;
         unsigned *bins = a.bins + (size_t)mblock * kBins * kM + lrow;
         const bool any = mblock * kM + quarter * 32 < a.T;          // a row of this warp is there
-        const int spare = max((kSlots - 16 - a.keep) / 2, 4);
+        constexpr int kSets = kN / 2 / 32;
         Run2 run{-INFINITY, 0.f, 0.f, 0.f};
-        float least = row < a.T ? -INFINITY : INFINITY;              // appended: what is above it
-        float tops[kN / 2 / 32], told[kN / 2 / 32];                  // of the four sets of 32 columns; last told
+        float least = row < a.T ? kAbsent : INFINITY;                // appended: what is above it
+        float reach = INFINITY;                  // the bound that the entries from base on all reach
+        int count = 0, base = 0, full_list = 0;
+        float tops[kSets], told[kSets];          // largest values of the four sets of 32 columns; last told
 #pragma unroll
-        for (int j = 0; j < kN / 2 / 32; ++j) tops[j] = told[j] = -INFINITY;
-        int count = 0;
+        for (int j = 0; j < kSets; ++j) tops[j] = told[j] = -INFINITY;
         uint32_t it = 0;
         for (int v = part; v < tiles; v += a.parts, ++it) {
             const uint32_t b = it & 1u;
-            // Before tiles 1, 2, 4, 8, .. each part takes a bound on what is worth a place in its list from
-            // the row's maxima that the parts have told each other (and before the first one, below). It may
-            // miss what others have just told: any such bound is a valid one, and the entries above
-            // the last are there in any case. The loads go out before the tile is there.
-            const bool look = any && it > 0 && (it & (it - 1u)) == 0u;
-            uint32_t o[kBins];
-            if (look) {
-#pragma unroll
-                for (int i = 0; i < kBins; ++i) o[i] = __ldcg(&bins[i * kM]);
-            }
             if (aborted(abort) || !wait_or_abort(&acc_full[b], (it >> 1) & 1u, abort)) break;
             tc_fence_after();
-            if (look) least = fmaxf(least, value_below(bins_bound(o, a.keep)));
             const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + b * kN + half * (kN / 2);
             const int col0 = v * a.width + half * (kN / 2);
             const int inside = min(cols, a.V - col0);               // columns that are there
-            auto load = [&](int c, float (&x)[32]) {
-                tmem_ld32(taddr + c, x);
-                if (c + 32 > inside) {
+            auto mask = [&](int j, uint32_t (&x)[32]) {
+                if (32 * j + 32 > inside) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        if (c + i >= inside) x[i] = -INFINITY;
+                        if (32 * j + i >= inside) x[i] = __float_as_uint(kAbsent);
                 }
             };
             auto tell = [&]() {
                 if (row >= a.T) return;
 #pragma unroll
-                for (int j = 0; j < kN / 2 / 32; ++j) {
+                for (int j = 0; j < kSets; ++j) {
                     if (tops[j] > told[j])
-                        atomicMax(&bins[(((part * kHalves + half) * 4 + j) % kBins) * kM], order_of(tops[j] + 0.f));
+                        atomicMax(&bins[(((part * kHalves + half) * kSets + j) % kBins) * kM], order_of(tops[j] + 0.f));
                     told[j] = tops[j];
                 }
             };
-            if (any && inside > 0) {
-                // the first tile: its maxima are told, its statistics taken while the others tell theirs, and
-                // its candidates only then. Passes: 0 statistics, 1 candidates, 2 both
-                if (it == 0) {
+            // Before the tiles 0, 1, 4, 16, .. each part takes a bound on what is worth a place in its list from
+            // the row's maxima that the parts have told each other. It may miss what others have just
+            // told: any such bound is a valid one, and the entries above the last are there in any case.
+            auto look = [&]() {
+                uint32_t o[kBins];
 #pragma unroll
-                    for (int j = 0; j < kN / 2 / 32; ++j) {
-                        if (32 * j < inside) {
-                            float x[32];
-                            load(32 * j, x);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) tops[j] = fmaxf(tops[j], x[i]);
-                        }
-                    }
-                    tell();
+                for (int i = 0; i < kBins; ++i) o[i] = __ldcg(&bins[i * kM]);
+                const uint32_t bound = bins_bound(o, a.keep);
+                const float below = value_below(bound);
+                if (below > least) {
+                    least = below;                                   // (those equal to the bound: by index)
+                    reach = value_of(bound);
+                    base = count;
                 }
-#pragma unroll 1
-                for (int pass = it == 0 ? 0 : 2; pass <= (it == 0 ? 1 : 2); ++pass) {
-                    if (pass == 1) {
+            };
+            // a set of columns: statistics (pass 0, 2), candidates (pass 1, 2)
+            auto take = [&](int j, uint32_t (&x)[32], int pass) {
+                mask(j, x);
+                float top[2];
 #pragma unroll
-                        for (int i = 0; i < kBins; ++i) o[i] = __ldcg(&bins[i * kM]);
-                        least = fmaxf(least, value_below(bins_bound(o, a.keep)));
-                    }
-#pragma unroll 1
-                    for (int j = 0; 32 * j < inside; ++j) {
-                        float x[32];
-                        load(32 * j, x);
-                        float top[2];
+                for (int h = 0; h < 2; ++h) {
+                    top[h] = __uint_as_float(x[16 * h]);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            top[h] = x[16 * h];
+                    for (int i = 1; i < 16; ++i) top[h] = fmaxf(top[h], __uint_as_float(x[16 * h + i]));
+                    if (pass != 0 && __any_sync(0xffffffffu, top[h] > least)) {
+                        if (count > kSlots - 16 && top[h] > least) {     // no room: the row is left to exact_kernel
+                            full_list = 1;
+                            least = INFINITY;
+                        }
 #pragma unroll
-                            for (int i = 1; i < 16; ++i) top[h] = fmaxf(top[h], x[16 * h + i]);
-                            if (pass != 0 && __any_sync(0xffffffffu, top[h] > least)) {
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) {
-                                    if (x[16 * h + i] > least) {                    // (+ 0: no -0 in a list)
-                                        list[count * kM] = make_uint2(__float_as_uint(x[16 * h + i] + 0.f),
-                                                                      (uint32_t)(col0 + 32 * j + 16 * h + i));
-                                        ++count;
-                                    }
-                                }
-                                if (__any_sync(0xffffffffu, count > kSlots - 16)) {
-                                    if (count > a.keep + spare) least = fmaxf(least, list_cut(list, count, a.keep, spare));
-                                    __syncwarp();
-                                }
+                        for (int i = 0; i < 16; ++i) {
+                            const float value = __uint_as_float(x[16 * h + i]);
+                            if (value > least) {                    // (+ 0: no -0 in a list)
+                                list[count * kM] = make_uint2(__float_as_uint(value + 0.f),
+                                                              (uint32_t)(col0 + 32 * j + 16 * h + i));
+                                ++count;
                             }
                         }
-                        const float both = fmaxf(top[0], top[1]);
-#pragma unroll
-                        for (int k = 0; k < kN / 2 / 32; ++k) tops[k] = fmaxf(tops[k], k == j ? both : -INFINITY);
-                        if (pass != 1) run2_add(run, x, both);
+                        // keep entries that reach the bound: more that only equal it come behind them by index
+                        if (count - base >= a.keep) least = fmaxf(least, reach < INFINITY ? reach : kAbsent);
                     }
                 }
-                if ((it & (it + 1u)) == 0u) tell();                  // the next tile looks
+                if (pass != 1) run2_add(run, x, fmaxf(top[0], top[1]));
+                return fmaxf(top[0], top[1]);
+            };
+            if (any && inside > 0) {
+                uint32_t xa[32], xb[32];
+                // the first tile: its maxima are told, its statistics taken while the others tell theirs, and
+                // its candidates only then
+                int pass = 2;
+                if (it == 0) {
+#pragma unroll
+                    for (int j = 0; j < kSets; ++j) {
+                        tmem_ld32(taddr + 32 * j, xa);
+                        tmem_wait(xa);
+                        mask(j, xa);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) tops[j] = fmaxf(tops[j], __uint_as_float(xa[i]));
+                        if (32 * j >= inside) tops[j] = -INFINITY;
+                    }
+                    tell();
+                    pass = 0;
+                } else if ((it & (it - 1u)) == 0u && (it & 0x55555555u)) {
+                    look();
+                }
+#pragma unroll 1
+                for (;; pass = 1) {
+                    if (pass == 1) look();
+                    // the next set is on its way while one is taken
+                    tmem_ld32(taddr, xa);
+#pragma unroll 1
+                    for (int j = 0; 32 * j < inside; j += 2) {
+                        tmem_wait(xa);
+                        tmem_ld32(taddr + 32 * (j + 1), xb);
+                        const float ta = take(j, xa, pass);
+                        tmem_wait(xb);
+                        if (j + 2 < kSets) tmem_ld32(taddr + 32 * (j + 2), xa);
+                        const float tb = 32 * (j + 1) < inside ? take(j + 1, xb, pass) : -INFINITY;
+#pragma unroll
+                        for (int k = 0; k < kSets; ++k)
+                            tops[k] = fmaxf(tops[k], k == j ? ta : k == j + 1 ? tb : -INFINITY);
+                    }
+                    tmem_wait(xa);
+                    if (pass != 0) break;
+                }
+                if ((it & (it + 1u)) == 0u && ((it + 1u) & 0x55555555u)) tell();     // the next tile looks
             }
             tc_fence_before();
             __syncwarp();
@@ -574,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (row < a.T) {
             const Soft s = run2_end(run);
-            a.stats[(size_t)slice * kM + lrow] = make_float4(s.m, s.s, s.w, __int_as_float(count));
+            a.stats[(size_t)slice * kM + lrow] = make_float4(s.m, s.s, s.w, __int_as_float(count | full_list << 16));
         }
     }
     __syncwarp();
@@ -658,7 +629,7 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     __shared__ int counts[kMaxLists];
     __shared__ Soft softs[kW];
     __shared__ float tau_s;
-    __shared__ int ncand;
+    __shared__ int ncand, lost;
     const int row = blockIdx.x, block = row / kM, lrow = row % kM;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int nlists = p.parts * kHalves;
@@ -668,9 +639,10 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     pdl_launch_dependents();
     pdl_wait();                                                     // score_kernel's lists and statistics
     if (tid == 0) {
-        ncand = 0;
+        ncand = lost = 0;
         tau_s = -INFINITY;
     }
+    __syncthreads();
 
     // statistics, in a fixed order
     Soft st = soft_none();
@@ -678,7 +650,9 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
         const float4 f = stats[(size_t)l * kM];
         st = soft_merge(st, Soft{f.x, f.y, f.z});
         peaks[l] = f.x;
-        counts[l] = min(max(__float_as_int(f.w), 0), kSlots);
+        const int w = __float_as_int(f.w);
+        counts[l] = min(w & 0xffff, kSlots);
+        if (w >> 16) lost = 1;                                      // (a list that could not hold all)
     }
     st = soft_warp(st);
     if (lane == 0) softs[warp] = st;
@@ -769,7 +743,7 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     // others' exact logits in place of the tensor cores'
     float err = 0.f;
     Soft sum{0.f, 0.f, 0.f};
-    const bool fine = st.m < INFINITY && st.m > -INFINITY && st.s < INFINITY && lead_n > 0;
+    const bool fine = st.m < INFINITY && st.m > -INFINITY && st.s < INFINITY && st.w > -INFINITY && lead_n > 0;
     if (fine) {
         sum.m = exact[0];
         for (int i = lane; i < lead_n; i += 32) {
@@ -823,7 +797,7 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     }
     // settled: there is nothing outside the candidates, or it cannot reach the n-th
     const float outside = lead_n > 0 ? top_value(lead[lead_n - 1]) : INFINITY;
-    const bool settled = fine && all <= kCand && lead_n >= p.n &&
+    const bool settled = fine && !lost && all <= kCand && lead_n >= p.n &&
                          (lead_n == p.V || (err == 0.f ? top_value(nth) >= outside
                                                        : top_value(nth) > outside + kMargin * err));
 #pragma unroll
