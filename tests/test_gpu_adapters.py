@@ -53,7 +53,8 @@ def check(bank, x, y, ids, out):
 
 SHAPES = [(1, 8, 1, 8, 1), (1, 2048, 768, 8, 4), (2, 64, 7, 16, 3), (3, 72, 100, 24, 2), (16, 256, 256, 32, 5),
           (17, 264, 257, 40, 5), (31, 1000, 333, 64, 3), (33, 3072, 768, 16, 40), (64, 768, 1000, 128, 9),
-          (65, 520, 65, 120, 4), (100, 128, 4097, 8, 7), (300, 96, 130, 48, 300), (513, 768, 96, 16, 2)]
+          (65, 520, 65, 120, 4), (100, 128, 4097, 8, 7), (300, 96, 130, 48, 300), (513, 768, 96, 16, 2),
+          (40, 8, 8, 8, 1100), (9001, 16, 24, 8, 37), (2500, 64, 40, 32, 900), (2, 4096, 20000, 64, 2)]
 
 
 @pytest.mark.parametrize("T,K,N,r,banks", SHAPES)
@@ -78,6 +79,30 @@ def test_row_patterns(dev, pattern, T):
 def test_head_sized_projection(dev):
     bank, x, y, ids = make(dev, 4, 1024, 248320, 16, 3, torch.float32, 5, [2, -1, 0, 2])
     check(bank, x, y, ids, bank.add(y, x, ids))
+
+
+def test_offsets_past_32_bits(dev):
+    """More than 2^31 outputs, and a bank of more than 2^31 values."""
+    from moe_offload_b200.adapters import AdapterBank
+    T, N = 8700, 248320
+    bank = AdapterBank.synthetic(2, 8, 8, N, dev)
+    x = torch.ones((T, 8), dtype=torch.bfloat16, device=dev)
+    y = torch.zeros((T, N), dtype=torch.float32, device=dev)
+    ids = torch.full((T,), -1, dtype=torch.int32, device=dev)
+    ids[T - 1], ids[0] = 1, 0
+    out = bank.add(y, x, ids, out=y)
+    rows = torch.tensor([0, T - 2, T - 1], device=dev)
+    check(bank, x[rows], torch.zeros((3, N), dtype=torch.float32, device=dev), ids[rows], out[rows])
+    del y, out
+    bank = AdapterBank(torch.zeros((70, 128, 64), dtype=torch.bfloat16, device=dev),
+                       torch.zeros((70, 248320, 128), dtype=torch.bfloat16, device=dev),
+                       torch.ones(70, dtype=torch.float32, device=dev))
+    bank.a[69] = 0.25
+    bank.b[69, -5:] = 0.5
+    x = torch.ones((3, 64), dtype=torch.bfloat16, device=dev)
+    y = torch.zeros((3, 248320), dtype=torch.float32, device=dev)
+    out = bank.add(y, x, torch.tensor([69, 68, -1], dtype=torch.int32, device=dev))
+    assert bool((out[0, -5:] == 1024.0).all()) and not bool(out[0, :-5].any()) and not bool(out[1:].any())
 
 
 def test_in_place_and_out(dev):

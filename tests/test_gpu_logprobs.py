@@ -285,7 +285,9 @@ def check_head(w, x, tg, n):
                                      (5, 1000, 1024, 32), (17, 4097, 520, 20), (127, 769, 256, 3), (128, 1024, 256, 20),
                                      (129, 513, 264, 5), (256, 2048, 128, 8), (257, 50021, 64, 20),
                                      (300, 33, 512, 32), (33, 32003, 2048, 0), (1, 248320, 1024, 20),
-                                     (640, 5000, 768, 20)])
+                                     (640, 5000, 768, 20),
+                                     (2049, 700, 64, 5), (2500, 1300, 72, 3), (6, 400, 8192, 4), (130, 512, 64, 32),
+                                     (40, 513, 64, 32)])
 def test_head_against_definition(dev, T, V, H, n):
     w, x, tg = head_case(dev, T, V, H, T + V + H)
     tg[T // 2] = -1
@@ -393,6 +395,57 @@ def test_head_captured_graphs_and_streams(dev):
     for o in outs:
         for a, b in zip(o, want):
             assert torch.equal(a, b)
+
+
+def test_head_same_bits_every_time(dev):
+    """What the parts of the vocabulary tell each other while they run does not show in the results."""
+    from moe_offload_b200.tokens import head_logprobs
+    for T, V, H in ((700, 20000, 128), (64, 60000, 64)):
+        w, x, tg = head_case(dev, T, V, H, 31)
+        w[5000:5200] = w[17]
+        want = head_logprobs(w, x, tg, 20)
+        for _ in range(6):
+            for a, b in zip(head_logprobs(w, x, tg, 20), want):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("order", [1, -1])
+def test_head_rising_and_falling(dev, order):
+    """Head rows in the order of their logits: every tile above (or below) all before it, so that no
+    bound taken on the way helps."""
+    T, V, H = 20, 80000, 64
+    g = torch.Generator(device=dev)
+    g.manual_seed(32)
+    base = torch.randn((1, H), generator=g, device=dev)
+    steps = torch.arange(V, device=dev)[:, None] * (order / V) + 2.0
+    w = (base * steps * 0.05).to(torch.bfloat16)
+    x = (base + 0.02 * torch.randn((T, H), generator=g, device=dev)).to(torch.bfloat16)
+    check_head(w, x, torch.arange(T, dtype=torch.int32, device=dev), 20)
+
+
+def test_offsets_past_32_bits(dev):
+    """More than 2^31 logits, and a head of more than 2^31 values."""
+    from moe_offload_b200.tokens import head_logprobs, token_logprobs
+    V, T = 248320, 8700
+    lg = torch.zeros((T, V), device=dev)
+    lg[T - 1, V - 1], lg[T - 1, 5], lg[T - 2, 7] = 9.0, 8.0, 7.0
+    tg = torch.zeros(T, dtype=torch.int32, device=dev)
+    tg[T - 1] = V - 1
+    r = token_logprobs(lg, tg, 2)
+    assert r.top_ids[T - 1].tolist() == [V - 1, 5] and r.top_ids[T - 2].tolist() == [7, 0]
+    rest = math.log1p(math.exp(-1.0) + (V - 2) * math.exp(-9.0))
+    assert abs(float(r.logprob[T - 1]) + rest) < RTOL * rest
+    assert abs(float(r.logprob[0]) + math.log(V)) < 5e-4
+    del lg
+    V, H = 1_050_000, 2048
+    w = torch.zeros((V, H), dtype=torch.bfloat16, device=dev)
+    w[V - 1, 0], w[V - 2, 1], w[3, 2] = 4.0, 3.0, 2.0
+    x = torch.ones((2, H), dtype=torch.bfloat16, device=dev)
+    r = head_logprobs(w, x, torch.tensor([V - 1, V - 2], dtype=torch.int32, device=dev), 3)
+    assert r.top_ids.tolist() == [[V - 1, V - 2, 3]] * 2
+    lse = math.log(math.exp(4.0) + math.exp(3.0) + math.exp(2.0) + V - 3)
+    assert abs(float(r.logprob[0]) - (4.0 - lse)) < HEAD_TOL * lse
+    assert abs(float(r.logprob[1]) - (3.0 - lse)) < HEAD_TOL * lse
 
 
 def test_refusals(dev):
