@@ -604,7 +604,7 @@ MOE_D float exact_logit(const uint16_t *w, const float4 *xs, int H) {
 
 constexpr int kCand = 1024;            // candidates that are ranked at once
 constexpr int kMaxLists = 512;         // lists of a row, at most
-constexpr int kGroups = 64;            // groups of threads whose maxima bound the candidates, with few lists
+constexpr int kGroups = 64;            // disjoint sets of entries whose maxima bound the candidates
 
 struct FinishArgs {
     const uint16_t *head, *x;          // x: this launch's first row
@@ -626,7 +626,8 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     constexpr int kW = kT / 32;
     extern __shared__ float4 xs[];                                  // the row (stage_row)
     __shared__ unsigned long long cand[kCand], lead[kKeep];
-    __shared__ float peaks[kMaxLists], exact[kKeep + 1];
+    __shared__ float peaks[kMaxLists], groups[kGroups], exact[kKeep + 1];
+    __shared__ unsigned long long bound_s;
     __shared__ int counts[kMaxLists];
     __shared__ Soft softs[kW];
     __shared__ float tau_s;
@@ -659,12 +660,11 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     if (lane == 0) softs[warp] = st;
     __syncthreads();
 
-    // the leading candidates: the keep-th largest of many disjoint maxima is a bound that keep entries
+    // the leading candidates: the keep-th largest of kGroups disjoint maxima is a bound that keep entries
     // reach. With enough lists their own maxima do, and only the lists that reach the bound are read;
-    // else those of kGroups groups of threads, which hold the entries of 2 lists a warp
+    // else those of the threads, which hold the entries of 2 lists a warp
     constexpr int kPer = kSlots / 32;
     const bool by_list = nlists >= 2 * p.keep;
-    const int npeaks = by_list ? nlists : kGroups;
     uint2 held[2][kPer];
     auto load_list = [&](int l, uint2 (&e)[kPer]) {
 #pragma unroll
@@ -672,7 +672,13 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
             e[i] = l < nlists && lane + 32 * i < counts[l] ? lists[((size_t)l * kSlots + lane + 32 * i) * kM]
                                                            : make_uint2(0xff800000u, 0u);          // -inf
     };
-    if (!by_list) {
+    if (by_list) {
+        if (tid < kGroups) {
+            float top = peaks[tid];
+            for (int l = tid + kGroups; l < nlists; l += kGroups) top = fmaxf(top, peaks[l]);
+            groups[tid] = top;
+        }
+    } else {
         float top = -INFINITY;
         for (int l = warp; l < nlists; l += 2 * kW) {
             load_list(l, held[0]);
@@ -683,45 +689,67 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
         }
 #pragma unroll
         for (int off = kT / kGroups / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        __syncthreads();                                            // (the lists' maxima are no longer needed)
-        if (tid % (kT / kGroups) == 0) peaks[tid / (kT / kGroups)] = top;
-        __syncthreads();
+        if (tid % (kT / kGroups) == 0) groups[tid / (kT / kGroups)] = top;
     }
-    for (int i = tid; i < npeaks; i += kT) {
-        const float mine = peaks[i];
+    __syncthreads();
+    if (tid < kGroups) {
+        const float mine = groups[tid];
         int r = 0;
-#pragma unroll 8
-        for (int j = 0; j < npeaks; ++j) r += (peaks[j] > mine || (peaks[j] == mine && j < i)) ? 1 : 0;
+#pragma unroll 16
+        for (int j = 0; j < kGroups; ++j) r += (groups[j] > mine || (groups[j] == mine && j < tid)) ? 1 : 0;
         if (r == p.keep - 1) tau_s = mine;
     }
     st = soft_warp(lane < kW ? softs[lane] : soft_none());
     __syncthreads();
     const float tau = tau_s;
-    const bool one_round = nlists <= 2 * kW;                  // held still has all entries
-    for (int l = warp; l < nlists; l += 2 * kW) {
-        if (by_list || !one_round) {
-            const bool a = !by_list || peaks[l] >= tau;
-            const bool b = l + kW < nlists && (!by_list || peaks[l + kW] >= tau);
-            if (!a && !b) continue;
-            load_list(a ? l : nlists, held[0]);
-            load_list(b ? l + kW : nlists, held[1]);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const float value = __uint_as_float(held[h][i].x);
-                if (value >= tau && value > -INFINITY) {
-                    const int at = atomicAdd(&ncand, 1);
-                    if (at < kCand) cand[at] = top_key(value, (int)held[h][i].y);
-                }
+    const bool one_round = nlists <= 2 * kW;                         // held still has all entries
+    // every entry that may reach tau
+    auto entries = [&](bool again, auto &&f) {
+        for (int l = warp; l < nlists; l += 2 * kW) {
+            if (by_list || !one_round || again) {
+                const bool a = !by_list || peaks[l] >= tau;
+                const bool b = l + kW < nlists && (!by_list || peaks[l + kW] >= tau);
+                if (!a && !b) continue;
+                load_list(a ? l : nlists, held[0]);
+                load_list(b ? l + kW : nlists, held[1]);
             }
-    }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const float value = __uint_as_float(held[h][i].x);
+                    if (value >= tau && value > -INFINITY) f(top_key(value, (int)held[h][i].y));
+                }
+        }
+    };
+    auto collect = [&](unsigned long long k) {
+        const int at = atomicAdd(&ncand, 1);
+        if (at < kCand) cand[at] = k;
+    };
+    entries(false, collect);
     __syncthreads();
+    if (ncand > kCand) {                         // ties at tau: the bound again, on (value, index) of each thread's best
+        unsigned long long best = 0ull;
+        entries(true, [&](unsigned long long k) { best = k > best ? k : best; });
+        __syncthreads();
+        cand[tid] = best;
+        if (tid == 0) ncand = 0;
+        __syncthreads();
+        int r = 0;
+        for (int j = 0; j < kT; ++j) r += (cand[j] > best || (cand[j] == best && j < tid)) ? 1 : 0;
+        if (r == p.keep - 1) bound_s = best;
+        __syncthreads();
+        const unsigned long long bound = bound_s;
+        entries(true, [&](unsigned long long k) {
+            if (k >= bound) collect(k);
+        });
+        __syncthreads();
+    }
     const int all = ncand, have = min(all, kCand);
     for (int i = tid; i < have; i += kT) {
         const unsigned long long k = cand[i];
         int r = 0;
+#pragma unroll 8
         for (int j = 0; j < have; ++j) r += cand[j] > k ? 1 : 0;
         if (r < p.keep) lead[r] = k;
     }

@@ -403,7 +403,9 @@ def test_head_same_bits_every_time(dev):
     for T, V, H in ((700, 20000, 128), (64, 60000, 64)):
         w, x, tg = head_case(dev, T, V, H, 31)
         w[5000:5200] = w[17]
+        x[3] = 0                                             # a padded row: every logit equal
         want = head_logprobs(w, x, tg, 20)
+        assert want.top_ids[3].tolist() == list(range(20))
         for _ in range(6):
             for a, b in zip(head_logprobs(w, x, tg, 20), want):
                 assert torch.equal(a, b)
