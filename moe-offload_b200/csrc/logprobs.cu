@@ -24,8 +24,6 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBatch = 4;              // chunks of 4 elements a thread has in flight
 constexpr int kCand = 256;             // elements above (or equal to) tau that are ranked at once
@@ -47,20 +45,21 @@ struct Row {
     MOE_D float at(int i) const { return (i >= 0 && i < V) ? __ldg(p + i) : -INFINITY; }
 };
 
-// kBatch chunks c, c + kThreads, ...; lo, hi: the chunks that lie wholly inside the row and this
+// kBatch chunks c, c + kT, ...; lo, hi: the chunks that lie wholly inside the row and this
 // CTA's part; end: the part's end
+template <int kT>
 MOE_D void load_batch(const Row &row, int c, int lo, int hi, int end, float (&v)[4 * kBatch]) {
-    if (c >= lo && c + (kBatch - 1) * kThreads < hi) {
+    if (c >= lo && c + (kBatch - 1) * kT < hi) {
         const float4 *q = reinterpret_cast<const float4 *>(row.p - row.a) + c;
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const float4 f = __ldg(q + j * kThreads);
+            const float4 f = __ldg(q + j * kT);
             v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
         }
     } else {
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const int cc = c + j * kThreads;
+            const int cc = c + j * kT;
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[4 * j + i] = cc < end ? row.at(4 * cc - row.a + i) : -INFINITY;
         }
@@ -74,7 +73,9 @@ struct WarpSum {
     int peaks;
 };
 
+template <int kT>
 struct Shared {
+    static constexpr int kWarps = kT / 32;
     float res[kWarps][32];                       // residue maxima of the warps
     float part_res[kMaxCluster][32];             // of the cluster's CTAs (written by them)
     // gathered in the cluster's first CTA: every warp's sums and the candidates of the row
@@ -98,8 +99,9 @@ MOE_D void append(unsigned long long *list, int *count, bool ok, unsigned long l
 }
 
 // scatters the m keys of a list to out by their rank (+ from) among themselves, ranks below n
+template <int kT>
 MOE_D void rank_out(const unsigned long long *list, int m, int from, int n, unsigned long long *out) {
-    for (int i = threadIdx.x; i < m; i += kThreads) {
+    for (int i = threadIdx.x; i < m; i += kT) {
         const unsigned long long k = list[i];
         int r = from;
         for (int j = 0; j < m; ++j) r += list[j] > k;
@@ -107,8 +109,11 @@ MOE_D void rank_out(const unsigned long long *list, int m, int from, int n, unsi
     }
 }
 
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobArgs p) {
-    __shared__ Shared sh;
+// kT threads a CTA (a cluster of several CTAs needs a warp for each: 512)
+template <int kT>
+__global__ void __launch_bounds__(kT) logprobs_kernel(LogprobArgs p) {
+    constexpr int kWarps = kT / 32;
+    __shared__ Shared<kT> sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -129,9 +134,9 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobArgs p) {
     float next = -INFINITY;
     int best = c0 + tid;
 #pragma unroll 1
-    for (int c = c0 + tid; c < c1; c += kThreads * kBatch) {
+    for (int c = c0 + tid; c < c1; c += kT * kBatch) {
         float v[4 * kBatch];
-        load_batch(row, c, lo, hi, c1, v);
+        load_batch<kT>(row, c, lo, hi, c1, v);
         float q[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -197,13 +202,13 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobArgs p) {
         const bool mine = peak >= tau && peak > -INFINITY;
         if (__ballot_sync(0xffffffffu, mine)) {
             float v[4 * kBatch];
-            if (mine) load_batch(row, best, lo, hi, c1, v);
+            if (mine) load_batch<kT>(row, best, lo, hi, c1, v);
 #pragma unroll
             for (int i = 0; i < 4 * kBatch; ++i) {
                 // (lanes that do not take part hold nothing: -inf is neither above tau nor equal to it)
                 const float x = mine ? v[i] : -INFINITY;
                 if (__ballot_sync(0xffffffffu, x >= tau && x > -INFINITY)) {
-                    const unsigned long long k = top_key(x, 4 * (best + (i >> 2) * kThreads) - row.a + (i & 3));
+                    const unsigned long long k = top_key(x, 4 * (best + (i >> 2) * kT) - row.a + (i & 3));
                     append(above, nabove, x > tau, k);
                     append(equal, nequal, x == tau && tau > -INFINITY, k);
                 }
@@ -214,13 +219,13 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobArgs p) {
                 const int owner = __ffs(who) - 1;
                 who &= who - 1;
                 const int ob = __shfl_sync(0xffffffffu, best, owner);
-                for (int c = c0 + 32 * warp + owner; c < c1; c += kThreads * 32) {
+                for (int c = c0 + 32 * warp + owner; c < c1; c += kT * 32) {
                     float x[4];
                     int at[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int cc = c + kThreads * (8 * j + (lane >> 2));
-                        const bool done = cc >= ob && cc < ob + kThreads * kBatch;       // the batch from above
+                        const int cc = c + kT * (8 * j + (lane >> 2));
+                        const bool done = cc >= ob && cc < ob + kT * kBatch;       // the batch from above
                         at[j] = 4 * cc - row.a + (lane & 3);
                         x[j] = cc < c1 && !done ? row.at(at[j]) : -INFINITY;
                     }
@@ -241,13 +246,13 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobArgs p) {
     if (n > 0) {
         const int na = sh.nabove, ne = sh.nequal;
         if (na <= kCand) {
-            rank_out(sh.above, na, 0, n, sh.out);
+            rank_out<kT>(sh.above, na, 0, n, sh.out);
             if (tau > -INFINITY && ne <= kCand) {
-                rank_out(sh.equal, ne, na, n, sh.out);
+                rank_out<kT>(sh.equal, ne, na, n, sh.out);
             } else {
                 // the first of the elements equal to tau, in index order (NaN counts as -inf)
                 const unsigned long long key0 = top_key(tau, 0) >> 32;
-                for (int i0 = 0, found = na; i0 < p.V && found < n; i0 += kThreads) {
+                for (int i0 = 0, found = na; i0 < p.V && found < n; i0 += kT) {
                     const int i = i0 + tid;
                     const unsigned long long k = i < p.V ? top_key(__ldg(base + i), i) : 0ull;
                     const bool ok = (k >> 32) == key0;
@@ -268,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobArgs p) {
             unsigned long long last = ~0ull;
             for (int r = 0; r < n; ++r) {
                 unsigned long long b = 0ull;
-                for (int i = tid; i < p.V; i += kThreads) {
+                for (int i = tid; i < p.V; i += kT) {
                     const unsigned long long k = top_key(__ldg(base + i), i);
                     if (k < last && k > b) b = k;
                 }
@@ -324,11 +329,22 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobArgs p) {
 
 int moe_token_logprobs_launch(const float *logits, int T, int V, const int32_t *targets, int n, float *logprob,
                               float *entropy, int32_t *top_ids, float *top_logprobs, void *stream) {
-    int parts = 1;
-    while (parts < kMaxCluster && (long long)T * parts < 148 && V / (2 * parts) >= 4096) parts *= 2;
+    // A CTA's work behind the pass over its elements is a chain of some 5,000 cycles, whatever it has read. So:
+    // a cluster only as far as the rows leave SMs free (T = 64, V = 248,320: 21.5 us with 4 CTAs a row, 25.6
+    // with 2, 29.7 with 8; T = 1: 10.2 with 8, 23.6 with 1), and fewer threads for many short rows
+    // (2,048 x 1,000: 17 us with 128, 25 with 256, 42 with 512; 2,048 x 50,021: 83, 87, 100;
+    // 2,048 x 248,320: 414, 357, 346).
+    int parts = 1, threads = 512;
+    if (V <= 16384) {
+        threads = T >= 148 ? 128 : 256;
+    } else if (T >= 296) {
+        threads = V <= 131072 ? 256 : 512;
+    } else {
+        while (parts < kMaxCluster && T * parts < 148 && V / (2 * parts) >= 14336) parts *= 2;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)T * (unsigned)parts);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.stream = as_stream(stream);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -337,7 +353,8 @@ int moe_token_logprobs_launch(const float *logits, int T, int V, const int32_t *
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;            // (a CTA alone is a cluster of one)
     const LogprobArgs p{logits, T, V, n, targets, logprob, entropy, top_ids, top_logprobs};
-    MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, logprobs_kernel, p));
+    auto kern = threads == 512 ? logprobs_kernel<512> : threads == 256 ? logprobs_kernel<256> : logprobs_kernel<128>;
+    MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
     return MOE_OK;
 }
 
