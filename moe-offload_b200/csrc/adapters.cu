@@ -77,7 +77,7 @@ struct Smem {
     unsigned member[kRows];            // which rows are of that kind
     int kinds, sums[kWarps];
     // gathering: the window's rows' adapters, and the places of each adapter's rows
-    uint16_t bin[kWindow];
+    uint16_t bin[kWindow], near[kWindow];
     int start[kMaxSort + 2], next[kMaxSort + 1];
 };
 
@@ -148,12 +148,24 @@ MOE_D int tile_rows(S &sh, const AdapterArgs &p, int tile, bool report) {
     bool mixed = false;
     if (p.sort) {
         int runs = 0;
-        for (int t = tid; t < wn; t += kThreads) {
-            const int id = ids[t];
-            runs += t == 0 || id != ids[t - 1] ? 1 : 0;
-            const bool in = id >= 0 && id < p.adapters;
-            if (!in && id != -1 && report) atomicOr(&g_moe_device_error, MOE_DEVERR_BAD_INPUT);
-            sh.bin[t] = (uint16_t)(in ? id : p.adapters);
+        constexpr int kB = 8;                    // ids a thread has in flight
+        for (int t0 = tid; t0 < wn; t0 += kB * kThreads) {
+            int id[kB], before[kB];
+#pragma unroll
+            for (int i = 0; i < kB; ++i) {
+                const int t = t0 + i * kThreads;
+                id[i] = t < wn ? __ldg(ids + t) : 0;
+                before[i] = t < wn && t > 0 ? __ldg(ids + t - 1) : ~id[i];
+            }
+#pragma unroll
+            for (int i = 0; i < kB; ++i) {
+                const int t = t0 + i * kThreads;
+                if (t >= wn) break;
+                runs += id[i] != before[i] ? 1 : 0;
+                const bool in = id[i] >= 0 && id[i] < p.adapters;
+                if (!in && id[i] != -1 && report) atomicOr(&g_moe_device_error, MOE_DEVERR_BAD_INPUT);
+                sh.bin[t] = (uint16_t)(in ? id[i] : p.adapters);
+            }
         }
         for (int i = tid; i <= p.adapters; i += kThreads) sh.next[i] = 0;
         runs = __reduce_add_sync(0xffffffffu, runs);
@@ -195,22 +207,40 @@ MOE_D int tile_rows(S &sh, const AdapterArgs &p, int tile, bool report) {
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
         if (lane == 0) sh.start[p.adapters + 1] = before;
-        __syncwarp();
-        for (int t0 = 0; t0 < wn; t0 += 32) {    // in row order, for the adapters that reach the tile
-            const int t = t0 + lane, b = t < wn ? sh.bin[t] : -1;
-            unsigned todo = __ballot_sync(0xffffffffu, b >= 0 && sh.start[b] < at + rows && sh.start[b + 1] > at);
-            while (todo) {
-                const int k = __shfl_sync(0xffffffffu, b, __ffs(todo) - 1);
-                const unsigned who = __ballot_sync(0xffffffffu, b == k);
-                todo &= ~who;
-                const int first = sh.next[k] - at, place = first + __popc(who & ((1u << lane) - 1u));
-                if (b == k && place >= 0 && place < rows) {
-                    sh.row[place] = w0 + t;
-                    sh.id[place] = b < p.adapters ? b : -1;
+    }
+    __syncthreads();
+    // the rows of the adapters that reach the tile: every warp lists those of its share of the window, in order
+    constexpr int kShare = kWindow / kWarps;
+    const int each = ((wn + kWarps - 1) / kWarps + 31) & ~31, t1 = min((warp + 1) * each, wn);
+    int found = 0;
+    for (int t0 = warp * each; t0 < t1; t0 += 32) {
+        const int t = t0 + lane, b = t < t1 ? sh.bin[t] : -1;
+        const bool near = b >= 0 && sh.start[b] < at + rows && sh.start[b + 1] > at;
+        const unsigned who = __ballot_sync(0xffffffffu, near);
+        if (near) sh.near[warp * kShare + found + __popc(who & ((1u << lane) - 1u))] = (uint16_t)t;
+        found += __popc(who);
+    }
+    if (lane == 0) sh.sums[warp] = found;
+    __syncthreads();
+    if (warp == 0) {                             // their places, in row order
+        for (int w = 0; w < kWarps; ++w) {
+            const int n = sh.sums[w];
+            for (int i0 = 0; i0 < n; i0 += 32) {
+                const int t = i0 + lane < n ? sh.near[w * kShare + i0 + lane] : -1, b = t >= 0 ? sh.bin[t] : -1;
+                unsigned todo = __ballot_sync(0xffffffffu, t >= 0);
+                while (todo) {
+                    const int k = __shfl_sync(0xffffffffu, b, __ffs(todo) - 1);
+                    const unsigned who = __ballot_sync(0xffffffffu, b == k);
+                    todo &= ~who;
+                    const int first = sh.next[k] - at, place = first + __popc(who & ((1u << lane) - 1u));
+                    if (b == k && place >= 0 && place < rows) {
+                        sh.row[place] = w0 + t;
+                        sh.id[place] = b < p.adapters ? b : -1;
+                    }
+                    __syncwarp();
+                    if (lane == 0) sh.next[k] = first + at + __popc(who);
+                    __syncwarp();
                 }
-                __syncwarp();
-                if (lane == 0) sh.next[k] = first + at + __popc(who);
-                __syncwarp();
             }
         }
     }
@@ -311,9 +341,14 @@ __global__ void __launch_bounds__(kThreads, kNT <= 8 ? 2 : 1) adapter_kernel(Ada
             const int r = 16 * m + (l >> 2) + 8 * h;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (c < S::kR && sh.id[r] >= 0) {
-                for (int k = 0; k < ctas; ++k) {
-                    const float4 o = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(&sh.u[r][c], k));
-                    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+                float4 o[kMaxCluster];
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; ++k)
+                    o[k] = k < ctas ? *reinterpret_cast<const float4 *>(cluster.map_shared_rank(&sh.u[r][c], k))
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; ++k) {
+                    v.x += o[k].x; v.y += o[k].y; v.z += o[k].z; v.w += o[k].w;
                 }
                 const float scale = __ldg(p.scale + sh.id[r]);
                 v.x *= scale; v.y *= scale; v.z *= scale; v.w *= scale;
