@@ -235,6 +235,12 @@ MOE_D uint32_t bins_bound(const uint32_t (&o)[kBins], int keep) {
     return lo;
 }
 
+// Clears the bins and lets score_kernel start meanwhile: only its epilogue needs them.
+__global__ void clear_kernel(uint4 *bins) {
+    pdl_launch_dependents();
+    bins[blockIdx.x * blockDim.x + threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 template <bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
     score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, ScoreArgs a) {
@@ -410,6 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp >= 2) {
         // ---- epilogue: thread = row, the tile's columns 0 .. 127 or the rest
+        pdl_wait();                              // the bins are clear
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const int cols = half ? a.width - kN / 2 : min(a.width, kN / 2);
         const int mblock = block * kCtas + rank, lrow = quarter * 32 + lane, row = mblock * kM + lrow;
@@ -957,12 +964,14 @@ int launch_score(const CUtensorMap &mx, const CUtensorMap &mw, const ScoreArgs &
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kPair ? 2 : 1;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kPair ? 2 : 1;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mx, mw, a));
     return MOE_OK;
 }
@@ -1022,7 +1031,9 @@ extern "C" int moe_head_logprobs(const void *head, int V, int H, const void *x, 
                           (uint32_t)xbox);
         if (rc) return rc;
         const ScoreArgs sa{rows, V, H, blocks, parts, width, xbox, n + kPad, lists, stats, bins, redo};
-        MOE_CUDA_TRY(cudaMemsetAsync(bins, 0, (size_t)blocks * ctas * kBins * kM * sizeof(unsigned), st));
+        constexpr int kClear = 256;                                  // 16 bytes a thread
+        clear_kernel<<<blocks * ctas * (kBins * kM / 4 / kClear), kClear, 0, st>>>(reinterpret_cast<uint4 *>(bins));
+        MOE_CUDA_TRY(cudaGetLastError());
         if ((rc = pl.paired ? launch_score<true>(mx, mw, sa, st) : launch_score<false>(mx, mw, sa, st))) return rc;
         int32_t *ids = n ? top_ids + (size_t)t0 * n : nullptr;
         float *tl = n ? top_logprobs + (size_t)t0 * n : nullptr;
