@@ -288,6 +288,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
         }
     }
+    {
+        // rows of X that no load will fill: zeros (their results are not read, but the tensor cores spend power
+        // on what is there)
+        const int row0 = (blockIdx.x / kCtas % a.blocks * kCtas + rank) * kM;
+        const int from = min(max((a.T - row0 + a.xbox - 1) / a.xbox, 0) * a.xbox, kM) * 128;
+        for (int s = 0; s < kStages; ++s)
+            for (int i = from + 16 * tid; i < (int)kABytes; i += 16 * kThreads)
+                *reinterpret_cast<uint4 *>(smem + (size_t)s * SL::kStageBytes + i) = make_uint4(0u, 0u, 0u, 0u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     tc_fence_before();
     if (kPair) pair.sync();                      // both CTAs' barriers are there
     else __syncthreads();
@@ -302,8 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- TMA, in each CTA for its own shared memory: 128 rows of X and the tile's rows of W (a pair: half of
         // them). Rows and columns of a box outside the arrays arrive as zeros, which costs
         // the TMA unit as much as data (one row in a box of 128 made the one-row case 1.4 times slower):
-        // a few rows come in boxes of 32, and rows of X in boxes wholly outside hold whatever was
-        // there, in lanes of the accumulator that nobody reads
+        // a few rows come in boxes of 32, and boxes of X wholly outside are left as they are
         const int row0 = (block * kCtas + rank) * kM;
         auto boxes = [&](int r0) { return min(max((a.T - r0 + a.xbox - 1) / a.xbox, 0), kM / a.xbox); };
         const int nx = boxes(row0), wrows = a.width / kCtas;
