@@ -461,16 +461,135 @@ __global__ void __launch_bounds__(kThreads, kNT <= 8 ? 2 : 1) adapter_kernel(Ada
     if (ctas > 1) cluster.barrier_wait();        // its own u stays until the others have read it
 }
 
+// One row a tile (a decode batch): a fragment of the tensor cores would hold 15 rows of nothing, so the
+// products run on the CUDA cores, in fp32 throughout. The cluster's CTAs split K, a warp takes two rank rows
+// at a time; then an output is 1, 2 or 4 lanes' work (32 ranks each at most), 4 outputs in flight a lane.
+template <bool kFp32>
+__global__ void __launch_bounds__(kThreads) adapter_row_kernel(AdapterArgs p) {
+    __shared__ __align__(16) float part[kMaxRank], u[kMaxRank];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int unit = blockIdx.x / ctas, t = unit / p.splits, split = unit % p.splits;
+    int id = __ldg(p.ids + t);
+    if (id < -1 || id >= p.adapters) {
+        if (tid == 0 && rank == 0 && split == 0) atomicOr(&g_moe_device_error, MOE_DEVERR_BAD_INPUT);
+        id = -1;
+    }
+    const int shares = p.splits * ctas, share = split * ctas + rank, per = ((p.N + shares - 1) / shares + 31) & ~31;
+    const int n0 = min(share * per, p.N), n1 = min(n0 + per, p.N);
+    const size_t row = (size_t)t * p.N;
+    if (id < 0) {                                // the same for the whole cluster; the row keeps its bits
+        if (p.out == p.y) return;
+        for (int n = n0 + tid; n < n1; n += kThreads) {
+            if (kFp32) static_cast<uint32_t *>(p.out)[row + n] = static_cast<const uint32_t *>(p.y)[row + n];
+            else static_cast<uint16_t *>(p.out)[row + n] = static_cast<const uint16_t *>(p.y)[row + n];
+        }
+        return;
+    }
+    auto dot8 = [](const uint4 &a, const float4 &x, const float4 &z, float s) {
+        s = fmaf(__uint_as_float(a.x << 16), x.x, s);
+        s = fmaf(__uint_as_float(a.x & 0xffff0000u), x.y, s);
+        s = fmaf(__uint_as_float(a.y << 16), x.z, s);
+        s = fmaf(__uint_as_float(a.y & 0xffff0000u), x.w, s);
+        s = fmaf(__uint_as_float(a.z << 16), z.x, s);
+        s = fmaf(__uint_as_float(a.z & 0xffff0000u), z.y, s);
+        s = fmaf(__uint_as_float(a.w << 16), z.z, s);
+        return fmaf(__uint_as_float(a.w & 0xffff0000u), z.w, s);
+    };
+    // ---- u = x . A^T
+    {
+        const int chunks = p.K / 8, each = (chunks + ctas - 1) / ctas;
+        const int c0 = rank * each, c1 = min(c0 + each, chunks);
+        const uint4 *xr = reinterpret_cast<const uint4 *>(p.x + (size_t)t * p.K);
+        for (int j = 2 * warp; j < p.rank; j += 2 * kWarps) {
+            const uint4 *a0 = reinterpret_cast<const uint4 *>(p.a + ((size_t)id * p.rank + j) * p.K);
+            const uint4 *a1 = a0 + chunks;
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
+            for (int c = c0 + lane; c < c1; c += 32) {
+                const uint4 q = __ldg(xr + c), v0 = __ldg(a0 + c), v1 = __ldg(a1 + c);
+                const float4 x = make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u),
+                                             __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u));
+                const float4 z = make_float4(__uint_as_float(q.z << 16), __uint_as_float(q.z & 0xffff0000u),
+                                             __uint_as_float(q.w << 16), __uint_as_float(q.w & 0xffff0000u));
+                s0 = dot8(v0, x, z, s0);
+                s1 = dot8(v1, x, z, s1);
+            }
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) {
+                s0 += __shfl_xor_sync(0xffffffffu, s0, off);
+                s1 += __shfl_xor_sync(0xffffffffu, s1, off);
+            }
+            if (lane == 0) {
+                part[j] = s0;
+                part[j + 1] = s1;
+            }
+        }
+    }
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
+    if (tid < p.rank) {
+        float o[kMaxCluster], s = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) o[k] = k < ctas ? *cluster.map_shared_rank(part + tid, k) : 0.f;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) s += o[k];
+        u[tid] = s * __ldg(p.scale + id);
+    }
+    __syncthreads();
+    if (ctas > 1) cluster.barrier_arrive();      // this CTA has read the others' sums (waited for at the end)
+    // ---- out = y + u . B^T
+    constexpr int kOut = 4, kQ = 4;              // outputs a lane, chunks of 8 ranks a lane and output
+    const int lanes = p.rank <= 32 ? 1 : p.rank <= 64 ? 2 : 4, mine = lane & (lanes - 1), sub = lane / lanes;
+    const int step = 32 / lanes, chunks = p.rank / 8;
+    for (int b0 = n0 + warp * kOut * step; b0 < n1; b0 += kWarps * kOut * step) {
+        uint4 w[kOut][kQ];
+        float y[kOut];
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) {
+            const int n = b0 + i * step + sub;
+            const uint4 *b = reinterpret_cast<const uint4 *>(p.b + ((size_t)id * p.N + n) * p.rank);
+#pragma unroll
+            for (int c = 0; c < kQ; ++c)
+                w[i][c] = n < n1 && mine + c * lanes < chunks ? __ldg(b + mine + c * lanes) : make_uint4(0u, 0u, 0u, 0u);
+            y[i] = n >= n1 || mine ? 0.f
+                   : kFp32         ? static_cast<const float *>(p.y)[row + n]
+                                   : bf16_bits_to_f32(static_cast<const uint16_t *>(p.y)[row + n]);
+        }
+        float s[kOut] = {};
+#pragma unroll
+        for (int c = 0; c < kQ; ++c) {
+            if (c * lanes >= chunks) break;
+            // (a lane behind the last chunk multiplies its zeros by the last one's u, which may not be finite)
+            const int at = mine + c * lanes;
+            const bool in = at < chunks;
+            const float4 x = *reinterpret_cast<const float4 *>(u + 8 * (in ? at : 0));
+            const float4 z = *reinterpret_cast<const float4 *>(u + 8 * (in ? at : 0) + 4);
+#pragma unroll
+            for (int i = 0; i < kOut; ++i) s[i] = in ? dot8(w[i][c], x, z, s[i]) : s[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) {
+            for (int off = 1; off < lanes; off <<= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], off);
+            const int n = b0 + i * step + sub;
+            if (n >= n1 || mine) continue;
+            if (kFp32) static_cast<float *>(p.out)[row + n] = y[i] + s[i];
+            else static_cast<uint16_t *>(p.out)[row + n] = f32_to_bf16_bits(y[i] + s[i]);
+        }
+    }
+    if (ctas > 1) cluster.barrier_wait();
+}
+
 bool overlap(const void *a, size_t na, const void *b, size_t nb) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
     return p < q + nb && q < p + na;
 }
 
-template <int kMT, int kNT, bool kFp32>
-int launch(const AdapterArgs &p, int ctas, cudaStream_t st) {
-    auto kern = adapter_kernel<kMT, kNT, kFp32>;
-    const size_t smem = sizeof(Smem<kMT, kNT, kFp32 ? 3 : 2>);
-    MOE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+template <typename Kern>
+int launch(Kern kern, size_t smem, const AdapterArgs &p, int ctas, cudaStream_t st) {
+    if (smem > 48 * 1024)
+        MOE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((p.T + p.rows - 1) / p.rows) * (unsigned)p.splits * (unsigned)ctas);
     cfg.blockDim = dim3(kThreads);
@@ -488,7 +607,8 @@ int launch(const AdapterArgs &p, int ctas, cudaStream_t st) {
 
 template <int kMT, int kNT>
 int dispatch_y(const AdapterArgs &p, int ctas, bool fp32, cudaStream_t st) {
-    return fp32 ? launch<kMT, kNT, true>(p, ctas, st) : launch<kMT, kNT, false>(p, ctas, st);
+    return fp32 ? launch(adapter_kernel<kMT, kNT, true>, sizeof(Smem<kMT, kNT, 3>), p, ctas, st)
+                : launch(adapter_kernel<kMT, kNT, false>, sizeof(Smem<kMT, kNT, 2>), p, ctas, st);
 }
 
 template <int kMT>
@@ -534,6 +654,9 @@ extern "C" int moe_adapter_add(const void *x, int T, int K, int N, const void *a
     if (N >= 16384) ctas = 2;
     while (tiles * ctas * (p.splits + 1) <= full && N / (ctas * (p.splits + 1)) >= kWarps * 64) ++p.splits;
     const bool wide = p.rows > 16;
+    if (p.rows == 1)
+        return y_fp32 ? launch(adapter_row_kernel<true>, 0, p, ctas, as_stream(stream))
+                      : launch(adapter_row_kernel<false>, 0, p, ctas, as_stream(stream));
     p.sort = p.rows > 1 && T > p.rows && adapters <= kMaxSort;
     return wide ? dispatch_rank<2>(p, ctas, y_fp32 != 0, as_stream(stream))
                 : dispatch_rank<1>(p, ctas, y_fp32 != 0, as_stream(stream));
