@@ -6,14 +6,17 @@
 // or the LM head's fp32 logits). One launch, no workspace: a cluster of CTAs takes a tile of rows and
 // a range of the N outputs. First u = x . A^T: the cluster's CTAs split K, their warps split it again,
 // and the partial sums (fp32) are added in a fixed order through distributed shared memory. Then each
-// CTA adds u . B^T to its share of the outputs. A tile goes through the adapters that its rows name, one
-// after another; rows of other adapters ride along in the products and are left out of the results.
-// Ids may come in any order: where they come mixed, tiles gather the rows of one adapter.
+// CTA adds u . B^T to its share of the outputs. A tile of several rows goes through the adapters that
+// its rows name, one after another; rows of other adapters ride along in the products and are left
+// out of the results. Ids may come in any order: where they come mixed, tiles gather the rows of one
+// adapter. A decode batch goes one row a tile, without the tensor cores (adapter_row_kernel).
 //
-// The products are 8 to 128 wide, far too little arithmetic per byte to be bound by the tensor cores
-// (rank 64: 60 FLOP per byte of x, y and out): mma.sync takes its operands from registers,
-// straight from 16-byte global loads. For that the K order inside a step is permuted alike in both
-// operands: a lane's consecutive elements fill its places of the fragments.
+// The products are 8 to 128 wide, far too little arithmetic per byte to need tcgen05's staging through
+// shared and tensor memory (rank 64: 60 FLOP per byte of x, y and out): mma.sync takes its operands from
+// registers, straight from 16-byte global loads. For that the K order inside a step is permuted
+// alike in both operands: a lane's consecutive elements fill its places of the fragments. What bounds
+// it is the chain of a tile's phases, 5 to 15 us of it, and beyond that mma.sync itself (0.4 a cycle an
+// SM): 2,048 rows of 768 -> 3,072, rank 64, 26 us, 0.18 of what x, y and out cost at the copy rate.
 //
 // u is carried into the second product as a sum of bf16 numbers: two of them (off by 2^-17 of u at most)
 // for bf16 outputs, whose own rounding is 2^-8, and three, which hold all of an fp32 number's 24 bits, for
@@ -600,7 +603,7 @@ int launch(Kern kern, size_t smem, const AdapterArgs &p, int ctas, cudaStream_t 
     attr[0].val.clusterDim.x = (unsigned)ctas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = ctas > 1 ? 1 : 0;             // (a CTA alone is a cluster of one)
     MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
     return MOE_OK;
 }
@@ -642,19 +645,29 @@ extern "C" int moe_adapter_add(const void *x, int T, int K, int N, const void *a
     AdapterArgs p{static_cast<const uint16_t *>(x), T, K, N, static_cast<const uint16_t *>(a),
                   static_cast<const uint16_t *>(b), scale, adapters, rank, ids, y, out, 16, 1, 0,
                   (ya & 15) == 0 && ((size_t)N * es) % 16 == 0};
-    // Rows a tile: as few as leave two CTAs an SM at four CTAs a tile, since the phases of a tile follow
-    // one another and only more tiles hide that (64 rows of 48 adapters, K = 3,072, N = 768: 6.6 us with
-    // one row a tile, 8.2 with two, 10 with four; 2,048 rows of rank 64: 26 us with 32, 31 with 16). A wide
-    // N (an LM head) is split over clusters of two, which repeat the small first product.
     const int full = 296;              // two CTAs on each of 148 SMs
-    p.rows = 1;
-    while (p.rows < 32 && (long long)((T + p.rows - 1) / p.rows) * 4 > full) p.rows *= 2;
+    // One row a tile while reading each row's own A and B costs less than what tiles cost on top: a decode
+    // batch, or up to 32 MB of them (K = 3,072, N = 768, rank 16, 30 adapters: 5.3 us against 8.6 for 100
+    // rows, 7.2 against 11.7 for 300; rank 64 of 2,048 x 2,048: 20 against 11.4 for 150). A cluster a
+    // row only where there are few (one row: 4.0 us with 8 CTAs, 64 rows: 5.0 with 1, 5.3 with 4).
+    const bool single = T <= full / 4 || (double)T * rank * ((double)K + N) * 2 <= 32e6;
+    int ctas;
+    if (single) {
+        p.rows = 1;
+        ctas = T * 8 <= full ? kMaxCluster : T < 64 ? 4 : 1;
+    } else {
+        // as few rows a tile as leave two CTAs an SM at four CTAs a tile, since the phases of a tile follow
+        // one another and only more tiles hide that (2,048 rows of rank 64: 26 us with 32 rows, 31 with 16)
+        p.rows = 2;
+        while (p.rows < 32 && (long long)((T + p.rows - 1) / p.rows) * 4 > full) p.rows *= 2;
+        ctas = (T + p.rows - 1) / p.rows * 8 <= full ? kMaxCluster : (T + p.rows - 1) / p.rows * 4 <= 2 * full ? 4 : 2;
+    }
+    // a wide N (an LM head) is split over clusters of two, which repeat the small first product
     const int tiles = (T + p.rows - 1) / p.rows;
-    int ctas = tiles * 8 <= full ? kMaxCluster : tiles * 4 <= 2 * full ? 4 : 2;
-    if (N >= 16384) ctas = 2;
-    while (tiles * ctas * (p.splits + 1) <= full && N / (ctas * (p.splits + 1)) >= kWarps * 64) ++p.splits;
+    if (N >= 16384 && ctas > 2) ctas = 2;
+    while ((long long)tiles * ctas * (p.splits + 1) <= full && N / (ctas * (p.splits + 1)) >= kWarps * 64) ++p.splits;
     const bool wide = p.rows > 16;
-    if (p.rows == 1)
+    if (single)
         return y_fp32 ? launch(adapter_row_kernel<true>, 0, p, ctas, as_stream(stream))
                       : launch(adapter_row_kernel<false>, 0, p, ctas, as_stream(stream));
     p.sort = p.rows > 1 && T > p.rows && adapters <= kMaxSort;

@@ -54,7 +54,11 @@ def check(bank, x, y, ids, out):
 SHAPES = [(1, 8, 1, 8, 1), (1, 2048, 768, 8, 4), (2, 64, 7, 16, 3), (3, 72, 100, 24, 2), (16, 256, 256, 32, 5),
           (17, 264, 257, 40, 5), (31, 1000, 333, 64, 3), (33, 3072, 768, 16, 40), (64, 768, 1000, 128, 9),
           (65, 520, 65, 120, 4), (100, 128, 4097, 8, 7), (300, 96, 130, 48, 300), (513, 768, 96, 16, 2),
-          (40, 8, 8, 8, 1100), (9001, 16, 24, 8, 37), (2500, 64, 40, 32, 900), (2, 4096, 20000, 64, 2)]
+          (40, 8, 8, 8, 1100), (9001, 16, 24, 8, 37), (2500, 64, 40, 32, 900), (2, 4096, 20000, 64, 2),
+          # tiles of several rows: more than 74 rows and 32 MB of A and B, counted once for each row
+          (75, 3072, 2048, 128, 11), (100, 3072, 2001, 64, 7), (130, 2048, 1030, 128, 5), (300, 1024, 1000, 64, 9),
+          (300, 3080, 768, 16, 20), (700, 2056, 777, 8, 3), (1100, 1000, 1003, 56, 2), (1500, 768, 513, 24, 37),
+          (2500, 512, 300, 16, 900), (2500, 264, 300, 40, 1100), (9001, 64, 72, 32, 37), (4100, 128, 33, 104, 50)]
 
 
 @pytest.mark.parametrize("T,K,N,r,banks", SHAPES)
@@ -65,14 +69,18 @@ def test_against_definition(dev, T, K, N, r, banks, dtype):
     check(bank, x, y, ids, out)
 
 
-@pytest.mark.parametrize("pattern", ["one", "none", "alternating", "runs", "last only", "each its own", "descending"])
-@pytest.mark.parametrize("T", [1, 15, 16, 48, 130])
-def test_row_patterns(dev, pattern, T):
+@pytest.mark.parametrize("pattern", ["one", "none", "alternating", "runs", "last only", "each its own", "descending",
+                                     "two thirds none"])
+@pytest.mark.parametrize("T,K,N,r", [(1, 384, 200, 16), (15, 384, 200, 16), (16, 384, 200, 16), (48, 384, 200, 16),
+                                     (130, 384, 200, 16), (77, 3072, 1024, 64), (130, 3072, 1024, 64),
+                                     (600, 2048, 520, 16), (2049, 256, 256, 32), (5000, 64, 64, 32)])
+def test_row_patterns(dev, pattern, T, K, N, r):
     banks = 7
     ids = {"one": [3] * T, "none": [-1] * T, "alternating": [t % 2 for t in range(T)],
            "runs": [t * 5 // T for t in range(T)], "last only": [-1] * (T - 1) + [6],
-           "each its own": [t % banks for t in range(T)], "descending": [banks - 1 - t * banks // T for t in range(T)]}
-    bank, x, y, ids = make(dev, T, 384, 200, 16, banks, torch.bfloat16, T, ids[pattern])
+           "each its own": [t % banks for t in range(T)], "descending": [banks - 1 - t * banks // T for t in range(T)],
+           "two thirds none": [t % banks if t % 3 == 0 else -1 for t in range(T)]}
+    bank, x, y, ids = make(dev, T, K, N, r, banks, torch.bfloat16, T, ids[pattern])
     check(bank, x, y, ids, bank.add(y, x, ids))
 
 
@@ -105,20 +113,22 @@ def test_offsets_past_32_bits(dev):
     assert bool((out[0, -5:] == 1024.0).all()) and not bool(out[0, :-5].any()) and not bool(out[1:].any())
 
 
-def test_in_place_and_out(dev):
-    bank, x, y, ids = make(dev, 50, 256, 301, 16, 4, torch.bfloat16, 6)
+@pytest.mark.parametrize("T,K,r", [(50, 256, 16), (150, 3072, 64)])
+def test_in_place_and_out(dev, T, K, r):
+    bank, x, y, ids = make(dev, T, K, 301, r, 4, torch.bfloat16, 6)
     want = bank.add(y, x, ids)
-    buf = torch.full((52, 301), 7.0, dtype=torch.bfloat16, device=dev)
-    out = bank.add(y, x, ids, out=buf[1:51])
+    buf = torch.full((T + 2, 301), 7.0, dtype=torch.bfloat16, device=dev)
+    out = bank.add(y, x, ids, out=buf[1:T + 1])
     assert out.data_ptr() == buf[1:].data_ptr() and torch.equal(out, want)
-    assert bool((buf[0] == 7).all()) and bool((buf[51] == 7).all())       # nothing written around it
+    assert bool((buf[0] == 7).all()) and bool((buf[T + 1] == 7).all())    # nothing written around it
     keep = y.clone()
     assert bank.add(keep, x, ids, out=keep) is keep and torch.equal(keep, want)
 
 
-def test_bad_ids_flagged_rows_kept(dev):
+@pytest.mark.parametrize("T,K,N,r", [(20, 64, 50, 8), (200, 3072, 1024, 64)])
+def test_bad_ids_flagged_rows_kept(dev, T, K, N, r):
     from moe_offload_b200 import _lib
-    bank, x, y, ids = make(dev, 20, 64, 50, 8, 3, torch.float32, 7, [0, 1, 2, 3, -2] + [-1] * 10 + [1] * 5)
+    bank, x, y, ids = make(dev, T, K, N, r, 3, torch.float32, 7, [0, 1, 2, 3, -2] + [-1] * (T - 10) + [1] * 5)
     _lib.call("moe_device_error", 1)
     out = bank.add(y, x, ids)
     torch.cuda.synchronize()
@@ -129,21 +139,23 @@ def test_bad_ids_flagged_rows_kept(dev):
     assert int(_lib.call("moe_device_error", 1)) == 0
 
 
-def test_infinities_stay_in_their_rows(dev):
+@pytest.mark.parametrize("T,K,N,r", [(40, 128, 96, 16), (120, 3072, 1024, 64)])
+def test_infinities_stay_in_their_rows(dev, T, K, N, r):
     """A row or an adapter with an inf or NaN changes no row that does not use it."""
-    bank, x, y, ids = make(dev, 40, 128, 96, 16, 4, torch.float32, 8, [t % 4 for t in range(40)])
+    bank, x, y, ids = make(dev, T, K, N, r, 4, torch.float32, 8, [t % 4 for t in range(T)])
     want = bank.add(y, x, ids)
     x[5, 3] = float("inf")
     x[9, 0] = float("nan")
     bank.a[2, 0, 0] = float("nan")
     got = bank.add(y, x, ids)
-    hit = (ids == 2) | (torch.arange(40, device=dev) == 5) | (torch.arange(40, device=dev) == 9)
+    hit = (ids == 2) | (torch.arange(T, device=dev) == 5) | (torch.arange(T, device=dev) == 9)
     assert torch.equal(got[~hit], want[~hit])
     assert not bool(torch.isfinite(got[hit]).all(dim=1).any())
 
 
-def test_streams_and_graphs(dev):
-    bank, x, y, ids = make(dev, 70, 512, 130, 32, 6, torch.bfloat16, 9)
+@pytest.mark.parametrize("T,K,r", [(70, 512, 32), (170, 3072, 64)])
+def test_streams_and_graphs(dev, T, K, r):
+    bank, x, y, ids = make(dev, T, K, 130, r, 6, torch.bfloat16, 9)
     want = bank.add(y, x, ids)
     s = torch.cuda.Stream(device=dev)
     s.wait_stream(torch.cuda.current_stream(dev))
