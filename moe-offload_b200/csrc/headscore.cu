@@ -200,7 +200,7 @@ MOE_D void run2_add(Run2 &a, uint32_t (&x)[32], float top) {
 MOE_D Soft run2_end(const Run2 &a) {
     if (a.m == -INFINITY) return Soft{a.m, a.s, 0.f};
     const float ln2 = 0.6931471805599453f;
-    const float d = (float)((double)a.r * 0.6931471805599453 - (double)a.m), f = fast_exp(d);
+    const float d = (float)((double)a.r * 0.6931471805599453 - (double)a.m), f = expf(d);
     return Soft{a.m, f * a.s, f * fmaf(ln2, a.w, d * a.s)};
 }
 
@@ -784,10 +784,13 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     __syncthreads();
     if (warp != 0) return;
 
-    // statistics relative to the exact logit of the leading candidate, which they leave out, with the
-    // others' exact logits in place of the tensor cores'
-    float err = 0.f;
-    Soft sum{0.f, 0.f, 0.f};
+    // Statistics relative to the exact logit of the leading candidate, which they leave out, with the
+    // others' exact logits in place of the tensor cores'. The tensor cores' accumulation rounds towards zero:
+    // logits come out smaller by a share that the candidates show (rho, some 1e-6), and the sums over
+    // the rest are moved by it to first order: sum a e^(a - m) is known, and the entropy's sum takes the
+    // rest's mean for its values.
+    float err = 0.f, gain = 0.f, size = 0.f;
+    Soft sum{0.f, 0.f, 0.f}, near_sum{0.f, 0.f, 0.f};
     const bool fine = st.m < INFINITY && st.m > -INFINITY && st.s < INFINITY && st.w > -INFINITY && lead_n > 0;
     if (fine) {
         sum.m = exact[0];
@@ -795,21 +798,33 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
             const float near = top_value(lead[i]), x = exact[i];
             err = fmaxf(err, fabsf(x - near));
             if (i > 0) {
+                gain += near < 0.f ? near - x : x - near;
+                size += fabsf(near);
                 const float dx = fmaxf(x - sum.m, kSoftFar), dn = fmaxf(near - sum.m, kSoftFar);
-                const float ex = fast_exp(dx), en = fast_exp(dn);
-                sum.s += ex - en;
-                sum.w += dx * ex - dn * en;
+                const float ex = expf(dx), en = expf(dn);
+                sum.s += ex;
+                sum.w += dx * ex;
+                near_sum.s += en;
+                near_sum.w += dn * en;
             }
         }
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) {
             sum.s += __shfl_xor_sync(0xffffffffu, sum.s, off);
             sum.w += __shfl_xor_sync(0xffffffffu, sum.w, off);
+            near_sum.s += __shfl_xor_sync(0xffffffffu, near_sum.s, off);
+            near_sum.w += __shfl_xor_sync(0xffffffffu, near_sum.w, off);
+            gain += __shfl_xor_sync(0xffffffffu, gain, off);
+            size += __shfl_xor_sync(0xffffffffu, size, off);
             err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, off));
         }
-        const float d = st.m - sum.m, f = fast_exp(d);
-        sum.s = fmaxf(fmaf(f, st.s, sum.s), 0.f);
-        sum.w += f * (st.w + d * st.s);
+        const float d = st.m - sum.m, f = expf(d);
+        const float rs = fmaf(f, st.s, -near_sum.s), rw = f * (st.w + d * st.s) - near_sum.w;     // the rest
+        if (rs > 0.f) {
+            const float rho = size > 0.f ? gain / size : 0.f, moved = rho * fmaf(sum.m, rs, rw);
+            sum.s += rs + moved;
+            sum.w += rw + moved * (1.f + rw / rs);
+        }
     } else {
         sum.m = __int_as_float(0x7fffffff);
     }

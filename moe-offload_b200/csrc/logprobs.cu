@@ -176,8 +176,8 @@ __global__ void __launch_bounds__(kT) logprobs_kernel(LogprobArgs p) {
 
     // ---- the sums relative to m; all its occurrences are left out and counted
     {
-        const float d = fmaxf(run.r - m, kSoftFar), f = fast_exp(d);
-        const float e = fmaxf(peak - m, kSoftFar), g = peak == m ? 0.f : fast_exp(e);
+        const float d = fmaxf(run.r - m, kSoftFar), f = expf(d);
+        const float e = fmaxf(peak - m, kSoftFar), g = peak == m ? 0.f : expf(e);
         WarpSum a{fmaf(f, run.s, g), fmaf(f, fmaf(d, run.s, run.w), e * g), peak == m};
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) {

@@ -20,7 +20,9 @@ struct Soft {
 constexpr float kSoftFar = -1000.f;
 
 // e^x and 2^x by the exponential unit, results below the smallest normal number 0 (without that, every
-// call carries three more instructions for them)
+// call carries three more instructions for them). The product with log2(e) is rounded: e^x is off by
+// |x| 2^-24 and more, alike for no two values, which a sum of many evens out. What scales a whole sum
+// takes expf.
 MOE_D float fast_pow2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -37,7 +39,7 @@ MOE_D Soft soft_merge(Soft a, Soft b) {
         a.s += b.s;
         return a;
     }
-    const float d = fmaxf(b.m - a.m, kSoftFar), e = fast_exp(d);
+    const float d = fmaxf(b.m - a.m, kSoftFar), e = expf(d);
     a.w += e * (b.w + d * (b.s + 1.f));
     a.s += (b.s + 1.f) * e;
     return a;
@@ -103,7 +105,7 @@ MOE_D void run_add(SoftRun &a, const float (&v)[kN], float top) {
 
 MOE_D Soft run_end(const SoftRun &a) {
     if (a.m == -INFINITY) return Soft{a.m, a.s, 0.f};
-    const float d = fmaxf(a.r - a.m, kSoftFar), f = fast_exp(d);
+    const float d = fmaxf(a.r - a.m, kSoftFar), f = expf(d);
     return Soft{a.m, f * a.s, f * (a.w + d * a.s)};
 }
 
