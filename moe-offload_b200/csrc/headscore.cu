@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     };
     if (by_list) {
         if (tid < kGroups) {
-            float top = peaks[tid];
+            float top = tid < nlists ? peaks[tid] : -INFINITY;
             for (int l = tid + kGroups; l < nlists; l += kGroups) top = fmaxf(top, peaks[l]);
             groups[tid] = top;
         }

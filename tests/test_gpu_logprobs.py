@@ -310,6 +310,18 @@ def test_head_peaked_rows(dev):
     assert float(r.logprob.max()) > -1e-3
 
 
+@pytest.mark.parametrize("T,V,H,n", [(2, 3006, 64, 5), (140, 3006, 64, 5), (600, 20000, 64, 5), (1100, 9000, 64, 3),
+                                     (2048, 5000, 64, 0), (2048, 5000, 64, 1)])
+def test_head_negative_logits(dev, T, V, H, n):
+    """Rows whose logits are all negative, at numbers of lists (two a part) below the 64 sets that bound
+    the candidates: a set without a list must count for nothing."""
+    w, x, tg = head_case(dev, T, V, H, T + V)
+    w[:, 0] = -8.0
+    x[:, 0] = 3.0
+    for k in range(2):                           # (the second run meets other leftovers in shared memory)
+        check_head(w, x, tg, n)
+
+
 def test_head_ties_and_padding_rows(dev):
     """Equal head rows (more than can be alternatives), rows of zeros (a padded batch: every logit
     equal), and the ids still the lowest first."""
