@@ -821,7 +821,11 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
         const float d = st.m - sum.m, f = expf(d);
         const float rs = fmaf(f, st.s, -near_sum.s), rw = f * (st.w + d * st.s) - near_sum.w;     // the rest
         if (rs > 0.f) {
-            const float rho = size > 0.f ? gain / size : 0.f, moved = rho * fmaf(sum.m, rs, rw);
+            // Each of the H / 16 steps loses at most 2^-23 of the sum so far. A larger share is no share: the
+            // candidates' sums cancel, their errors have nothing to do with their size, and the rest stays.
+            const float most = (float)((p.H + 15) / 16) * 1.1920929e-7f;
+            const float rho = fabsf(gain) <= most * size && size > 0.f ? gain / size : 0.f;
+            const float moved = rho * fmaf(sum.m, rs, rw);
             sum.s += rs + moved;
             sum.w += rw + moved * (1.f + rw / rs);
         }

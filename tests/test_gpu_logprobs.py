@@ -322,6 +322,24 @@ def test_head_negative_logits(dev, T, V, H, n):
         check_head(w, x, tg, n)
 
 
+def test_head_cancelling_leaders(dev):
+    """The leading logits are sums that cancel to 0 and that the tensor cores leave a little beside it: their
+    errors are no share of their size, and the entries at -10 (a fifth of the sum) must not be moved by one.
+    The 13 = n + 8 leading ones are summed again exactly and the others are single products, so what is left is
+    the arithmetic that HEAD_TOL counts."""
+    V, H, n = 60000, 1024, 5
+    g = torch.Generator().manual_seed(77)
+    w = torch.zeros((V, H))
+    w[:, 0] = -10.0
+    half = torch.randn((n + 8, H // 2), generator=g) * 2.0 ** torch.randint(-14, 7, (n + 8, H // 2), generator=g)
+    half = half.bfloat16().float()
+    w[100:100 + n + 8] = torch.cat((half, -half.flip(1)), 1)
+    w = w.bfloat16().to(dev)
+    for T in (1, 3, 140):
+        x = torch.ones((T, H), dtype=torch.bfloat16, device=dev)
+        check_head(w, x, torch.arange(T, dtype=torch.int32, device=dev) + 99, n)
+
+
 def test_head_ties_and_padding_rows(dev):
     """Equal head rows (more than can be alternatives), rows of zeros (a padded batch: every logit
     equal), and the ids still the lowest first."""
