@@ -12,7 +12,7 @@
 // adapter. A decode batch goes one row a tile, without the tensor cores (adapter_row_kernel).
 //
 // The products are 8 to 128 wide, far too little arithmetic per byte to need tcgen05's staging through
-// shared and tensor memory (rank 64: 60 FLOP per byte of x, y and out): mma.sync takes its operands from
+// shared and tensor memory (rank 64: 36 FLOP per byte of x, y and out): mma.sync takes its operands from
 // registers, straight from 16-byte global loads. For that the K order inside a step is permuted
 // alike in both operands: a lane's consecutive elements fill its places of the fragments. What bounds
 // it is the chain of a tile's phases, 5 to 15 us of it, and beyond that mma.sync itself (0.4 a cycle an

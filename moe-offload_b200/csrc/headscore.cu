@@ -9,6 +9,7 @@
 //                  by side, so the head is read from HBM once and from L2 after that. Up to 128 rows,
 //                  where the head's bytes are the bound, every CTA works alone on tiles of 128 rows: a
 //                  pair would take twice as long for the same bytes.
+//                  The parts share a bound on candidates through kBins maxima a row (clear_kernel).
 //   finish_kernel  one CTA per row: joins the parts, sums the leading candidates' and the target's
 //                  logits again in 64 bits, exactly as the LM head does, corrects the statistics by
 //                  them and orders the alternatives.
@@ -159,8 +160,9 @@ MOE_D float value_below(uint32_t o) { return o > 0x00800000u ? value_of(o - (o =
 
 // A row's statistics while its tiles go by, in steps of 2: sums over 2^(x log2(e) - r) with r a whole
 // number near log2(e) times the largest value m, which the sums leave out (as SoftRun does). r is exact,
-// rescaling by it too, and one FMA makes an exponent. The fp32 constant is 1.3e-8 off, which moves the
-// sums by 1.3e-8 |m| relative to e^m: 1e-5 at a logit of 1,000.
+// rescaling by it too, and one FMA makes an exponent. The fp32 constant is 1.3e-8 off: run2_end takes m by the
+// same constant, so that only the differences from m see it. (2^t overflows where the FMA and r may lie 128
+// apart: logits from 2^30 on.)
 struct Run2 {
     float m, r, s, w;                  // w: sum of t 2^t, t the exponents
 };
@@ -200,7 +202,8 @@ MOE_D void run2_add(Run2 &a, uint32_t (&x)[32], float top) {
 MOE_D Soft run2_end(const Run2 &a) {
     if (a.m == -INFINITY) return Soft{a.m, a.s, 0.f};
     const float ln2 = 0.6931471805599453f;
-    const float d = (float)((double)a.r * 0.6931471805599453 - (double)a.m), f = expf(d);
+    // r and m on the same scale, that of the rounded log2(e)
+    const float d = (float)(((double)a.r - (double)a.m * (double)kLog2e) * 0.6931471805599453), f = expf(d);
     return Soft{a.m, f * a.s, f * fmaf(ln2, a.w, d * a.s)};
 }
 

@@ -340,6 +340,23 @@ def test_head_cancelling_leaders(dev):
         check_head(w, x, torch.arange(T, dtype=torch.int32, device=dev) + 99, n)
 
 
+@pytest.mark.parametrize("size", [1e3, 2.0 ** 20, -2.0 ** 20, 2.0 ** 29])
+def test_head_large_logits(dev, size):
+    """Logits of a large size, each a single product (the tensor cores lose nothing): 6 equal ones and
+    3,000 that lie a step of bf16 below, or all equal. What lies below is nothing next to them, the equal
+    ones' log-probability is -log of their number."""
+    V, H = 3006, 64
+    for equal in (6, V):
+        w = torch.zeros((V, H))
+        w[:, 0] = size * (0.5 if size > 0 else 2.0)
+        w[1000:1006, 0] = size
+        if equal == V:
+            w[:, 0] = size
+        x = torch.zeros((2, H))
+        x[:, 0] = 1.0
+        check_head(w.bfloat16().to(dev), x.bfloat16().to(dev), torch.tensor([1002, 1005], dtype=torch.int32, device=dev), 5)
+
+
 def test_head_ties_and_padding_rows(dev):
     """Equal head rows (more than can be alternatives), rows of zeros (a padded batch: every logit
     equal), and the ids still the lowest first."""
