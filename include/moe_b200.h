@@ -784,8 +784,9 @@ size_t moe_head_logprobs_workspace_bytes(int T, int V, int n);
  * The same outputs straight from bf16 rows x [T, H] and the bf16 head [V, H] (both 16-byte aligned,
  * H a multiple of 8 up to 8192; any T): prompt scoring without [T, V] logits in memory. The ids are
  * in the order of the logits moe_lm_head_logits computes, and the logits of the targets and of the
- * alternatives are those. A row with a logit that is not finite has no distribution. Calls that share
- * a workspace must not overlap on the GPU.
+ * alternatives are those. A row with a logit that is not finite has no distribution. The sums over the
+ * other logits take the tensor cores' own, which are off by up to their size times H / 16 * 2^-23; logits
+ * from 2^30 in size on may give NaN. Calls that share a workspace must not overlap on the GPU.
  */
 int moe_head_logprobs(const void *head, int V, int H, const void *x, int T, const int32_t *targets, int n,
                       float *logprob, float *entropy, int32_t *top_ids, float *top_logprobs, void *workspace,

@@ -17,6 +17,9 @@
 //                  holds, values that are not finite): all V logits in 64 bits. It reads the rows'
 //                  number and ends when there are none.
 //
+// B200, head 248,320 x 3,072: one row 242 us (0.98 of the copy rate), 256 rows 343 us, 2,048 rows 2.25 to 2.7 ms by
+// the power limit (2.20 ms at the sustained rate of the tensor cores).
+//
 // A tensor-core logit carries the rounding of H / 16 fp32 accumulations. That moves the log of the sum
 // of e^logit by the probability-weighted mean of those errors, a few 1e-7; it must not move an id or a
 // logit that is returned, hence the second sum. A candidate list is enough when the n-th exact logit

@@ -11,6 +11,7 @@
 // threads whose own maximum reaches tau look at their elements again (at one batch of 16, unless
 // another batch of theirs reaches tau too); the few that reach it are ranked by counting. No
 // running list, no sort.
+// B200, n = 20: 512 rows of 248,320 100 us (0.78 of the copy rate), one row 9.9 us, which is latency.
 // Ties at tau (a mask that leaves fewer than n tokens, a row of equal logits) are taken in index
 // order from the start of the row; a row whose large elements crowd into fewer than n residues
 // takes n passes.

@@ -103,12 +103,6 @@ MOE_D void run_add(SoftRun &a, const float (&v)[kN], float top) {
     }
 }
 
-MOE_D Soft run_end(const SoftRun &a) {
-    if (a.m == -INFINITY) return Soft{a.m, a.s, 0.f};
-    const float d = fmaxf(a.r - a.m, kSoftFar), f = expf(d);
-    return Soft{a.m, f * a.s, f * (a.w + d * a.s)};
-}
-
 // ------------------------------------------------------------------ order of the entries
 
 // Order-preserving 64-bit key of (value, index): larger value first, equal values the lower
@@ -125,19 +119,10 @@ MOE_D float top_value(unsigned long long k) {
 }
 MOE_D int top_index(unsigned long long k) { return (int)(0xffffffffu - (uint32_t)(k & 0xffffffffull)); }
 
-// Bitonic networks over one key per lane, descending with the lane.
+// A step of a bitonic network over one key per lane.
 MOE_D unsigned long long top_cmpx(unsigned long long k, int off, bool keep_max) {
     const unsigned long long o = __shfl_xor_sync(0xffffffffu, k, off);
     return (k > o) == keep_max ? k : o;
-}
-MOE_D unsigned long long top_sort(unsigned long long k) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int off = size >> 1; off > 0; off >>= 1)
-            k = top_cmpx(k, off, ((lane & off) == 0) == ((lane & size) == 0 || size == 32));
-    return k;
 }
 // a, b sorted descending over the lanes: the 32 largest of both, sorted descending
 MOE_D unsigned long long top_merge(unsigned long long a, unsigned long long b) {
