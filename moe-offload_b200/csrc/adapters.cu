@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, kNT <= 8 ? 2 : 1) adapter_kernel(Ada
     for (int i = tid; i < S::kRows * S::kR; i += kThreads) {
         const int r = i / S::kR, c = i % S::kR;
         float s = 0.f;
-        if (sh.id[r] >= 0) {
+        if (sh.id[r] >= 0 && c < p.rank) {       // (behind the rank: 0 times what x holds, an infinity too)
 #pragma unroll
             for (int w = 0; w < S::kWK; ++w) s += sh.part[w][r][c];
         }

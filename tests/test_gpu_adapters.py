@@ -205,3 +205,23 @@ def test_empty_batch_and_refusals(dev):
     wide = torch.zeros((9, 64), dtype=torch.bfloat16, device=dev)
     with pytest.raises(MoeError):
         bank.add(wide[:4], x, ids, out=wide[1:5])            # out over a part of y
+
+
+@pytest.mark.parametrize("rank", [8, 16, 24, 40, 72])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [2, 2000])
+def test_infinite_inputs_stay_infinite(rank, dtype, T):
+    """An infinity in x with a and b positive: the row's outputs are +inf by the formula, and no NaN comes from
+    places behind the rank. Two rows go one a tile, 2,000 in tiles of several; the other rows stay finite."""
+    from moe_offload_b200.adapters import AdapterBank
+    dev = torch.device("cuda:0")
+    K = N = 1024
+    bank = AdapterBank(torch.full((2, rank, K), 0.01, dtype=torch.bfloat16, device=dev),
+                       torch.full((2, N, rank), 0.5, dtype=torch.bfloat16, device=dev),
+                       torch.ones(2, device=dev))
+    x = torch.ones((T, K), dtype=torch.bfloat16, device=dev)
+    x[1, 3] = float("inf")
+    y = torch.zeros((T, N), dtype=dtype, device=dev)
+    out = bank.add(y, x, (torch.arange(T, device=dev) % 2).int())
+    assert torch.isposinf(out[1]).all()
+    assert torch.isfinite(out[torch.arange(T, device=dev) != 1]).all()
