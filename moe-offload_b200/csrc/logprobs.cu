@@ -177,7 +177,8 @@ __global__ void __launch_bounds__(kT) logprobs_kernel(LogprobArgs p) {
 
     // ---- the sums relative to m; all its occurrences are left out and counted
     {
-        const float d = fmaxf(run.r - m, kSoftFar), f = expf(d);
+        // (a thread without a finite logit has no reference: nothing, or a NaN, to pass on)
+        const float d = fmaxf(run.r - m, kSoftFar), f = peak > -INFINITY ? expf(d) : 0.f;
         const float e = fmaxf(peak - m, kSoftFar), g = peak == m ? 0.f : expf(e);
         WarpSum a{fmaf(f, run.s, g), fmaf(f, fmaf(d, run.s, run.w), e * g), peak == m};
 #pragma unroll
