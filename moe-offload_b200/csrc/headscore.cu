@@ -13,9 +13,8 @@
 //   finish_kernel  one CTA per row: joins the parts, sums the leading candidates' and the target's
 //                  logits again in 64 bits, exactly as the LM head does, corrects the statistics by
 //                  them and orders the alternatives.
-//   exact_kernel   rows whose order the candidates do not settle (more near-equal logits than a list
-//                  holds, values that are not finite): all V logits in 64 bits. It reads the rows'
-//                  number and ends when there are none.
+//   exact_kernel   rows whose order the candidates do not settle (near-equal logits, values that are not
+//                  finite): all V logits in 64 bits. It reads the rows' number and ends when there are none.
 //
 // B200, head 248,320 x 3,072: one row 242 us (0.98 of the copy rate), 256 rows 343 us, 2,048 rows 2.25 to 2.7 ms by
 // the power limit (2.20 ms at the sustained rate of the tensor cores).
@@ -45,7 +44,7 @@ constexpr int kHalves = 2;
 constexpr uint32_t kABytes = kM * 128;
 constexpr uint32_t kTmemCols = 512;    // two accumulators of kN columns: one fills while one is read
 
-constexpr int kSlots = 160;            // a row's list in one part: a first tile whole (128), and some
+constexpr int kSlots = 160;            // a row's list in one part: a first tile whole (128), and 32 more
 constexpr int kPad = 8;                // kept beyond n, to tell whether the order of the n is settled
 constexpr int kKeep = kTopMax + kPad;  // at most
 constexpr int kBins = 64;              // disjoint maxima of a row, for a bound on its keep-th largest logit
@@ -239,6 +238,50 @@ MOE_D uint32_t bins_bound(const uint32_t (&o)[kBins], int keep) {
         }
     }
     return lo;
+}
+
+// A row's list cut to its keep largest entries (equal ones: the lower index), in their order, by the whole
+// warp: list is the row's own, of n >= keep entries. Returns the smallest value kept. What is dropped, and what
+// comes later and does not exceed that value, has keep entries of this list before it, so it is none of the
+// row's keep largest. Out of line: few rows need it (a part's entries above the bound outnumber its list: a
+// vocabulary in blocks or in order, or a first tile before the other parts have told their maxima).
+__device__ __noinline__ float cut_list(uint2 *list, int n, int keep) {
+    constexpr int kPer = kSlots / 32;
+    const int lane = threadIdx.x & 31;
+    uint2 e[kPer];
+    uint32_t o[kPer];
+    __syncwarp();                                 // the row's lane has written its entries
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int at = lane + 32 * i;
+        e[i] = at < n ? list[at * kM] : make_uint2(0u, 0u);
+        o[i] = at < n ? order_of(__uint_as_float(e[i].x)) : 0u;
+    }
+    uint32_t t = 0u;                              // the largest image that keep entries reach
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t u = t | (1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) c += o[i] >= u ? 1 : 0;
+        if (__reduce_add_sync(0xffffffffu, c) >= keep) t = u;
+    }
+    int over = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) over += o[i] > t ? 1 : 0;
+    int ties = keep - __reduce_add_sync(0xffffffffu, over), to = 0;
+    const unsigned before = (1u << lane) - 1u;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {              // (all entries are in registers: they may move up in place)
+        const unsigned equal = __ballot_sync(0xffffffffu, o[i] == t);
+        const bool in = o[i] > t || (o[i] == t && __popc(equal & before) < ties);
+        ties -= min(ties, __popc(equal));
+        const unsigned who = __ballot_sync(0xffffffffu, in);
+        if (in) list[(to + __popc(who & before)) * kM] = e[i];
+        to += __popc(who);
+    }
+    __syncwarp();
+    return value_of(t);
 }
 
 // Clears the bins and lets score_kernel start meanwhile: only its epilogue needs them.
@@ -443,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         Run2 run{-INFINITY, 0.f, 0.f, 0.f};
         float least = row < a.T ? kAbsent : INFINITY;                // appended: what is above it
         float reach = INFINITY;                  // the bound that the entries from base on all reach
-        int count = 0, base = 0, full_list = 0;
+        int count = 0, base = 0;
         float tops[kSets], told[kSets];          // largest values of the four sets of 32 columns; last told
 #pragma unroll
         for (int j = 0; j < kSets; ++j) tops[j] = told[j] = -INFINITY;
@@ -496,10 +539,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 1; i < 16; ++i) top[h] = fmaxf(top[h], __uint_as_float(x[16 * h + i]));
                     if (pass != 0 && __any_sync(0xffffffffu, top[h] > least)) {
-                        if (count > kSlots - 16 && top[h] > least) {     // no room: the row is left to exact_kernel
-                            full_list = 1;
-                            least = INFINITY;
-                        }
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const float value = __uint_as_float(x[16 * h + i]);
@@ -511,6 +550,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         // keep entries that reach the bound: more that only equal it come behind them by index
                         if (count - base >= a.keep) least = fmaxf(least, reach < INFINITY ? reach : kAbsent);
+                    }
+                }
+                // 32 more have to fit
+                for (unsigned full = __ballot_sync(0xffffffffu, count > kSlots - 32); full;
+                     full &= full - 1) {
+                    const int of = __ffs(full) - 1;
+                    const float bound = cut_list(list + (of - lane), __shfl_sync(0xffffffffu, count, of), a.keep);
+                    if (lane == of) {
+                        count = base = a.keep;
+                        least = fmaxf(least, bound);
                     }
                 }
                 if (pass != 1) run2_add(run, x, fmaxf(top[0], top[1]));
@@ -567,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (row < a.T) {
             const Soft s = run2_end(run);
-            a.stats[(size_t)slice * kM + lrow] = make_float4(s.m, s.s, s.w, __int_as_float(count | full_list << 16));
+            a.stats[(size_t)slice * kM + lrow] = make_float4(s.m, s.s, s.w, __int_as_float(count));
         }
     }
     __syncwarp();
@@ -653,7 +702,7 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     __shared__ int counts[kMaxLists];
     __shared__ Soft softs[kW];
     __shared__ float tau_s;
-    __shared__ int ncand, lost;
+    __shared__ int ncand;
     const int row = blockIdx.x, block = row / kM, lrow = row % kM;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int nlists = p.parts * kHalves;
@@ -663,7 +712,7 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     pdl_launch_dependents();
     pdl_wait();                                                     // score_kernel's lists and statistics
     if (tid == 0) {
-        ncand = lost = 0;
+        ncand = 0;
         tau_s = -INFINITY;
     }
     __syncthreads();
@@ -674,9 +723,7 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
         const float4 f = stats[(size_t)l * kM];
         st = soft_merge(st, Soft{f.x, f.y, f.z});
         peaks[l] = f.x;
-        const int w = __float_as_int(f.w);
-        counts[l] = min(w & 0xffff, kSlots);
-        if (w >> 16) lost = 1;                                      // (a list that could not hold all)
+        counts[l] = min(__float_as_int(f.w), kSlots);
     }
     st = soft_warp(st);
     if (lane == 0) softs[warp] = st;
@@ -867,7 +914,7 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     }
     // settled: there is nothing outside the candidates, or it cannot reach the n-th
     const float outside = lead_n > 0 ? top_value(lead[lead_n - 1]) : INFINITY;
-    const bool settled = fine && !lost && all <= kCand && lead_n >= p.n &&
+    const bool settled = fine && all <= kCand && lead_n >= p.n &&
                          (lead_n == p.V || (err == 0.f ? top_value(nth) >= outside
                                                        : top_value(nth) > outside + kMargin * err));
 #pragma unroll
