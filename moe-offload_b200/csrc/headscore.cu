@@ -808,13 +808,39 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
         for (int j = 0; j < kT; ++j) r += (cand[j] > best || (cand[j] == best && j < tid)) ? 1 : 0;
         if (r == p.keep - 1) bound_s = best;
         __syncthreads();
-        const unsigned long long bound = bound_s;
+        unsigned long long bound = bound_s;
         entries(true, [&](unsigned long long k) {
             if (k >= bound) collect(k);
         });
         __syncthreads();
+        if (ncand > kCand) {                     // crowded in a few threads: a bound bit by bit (keys differ)
+            bound = 0ull;
+            int reach = 0;
+            for (int bit = 63; bit >= 0 && !(reach >= p.keep && reach <= kCand); --bit) {
+                const unsigned long long u = bound | (1ull << bit);
+                int c = 0;
+                entries(true, [&](unsigned long long k) { c += k >= u ? 1 : 0; });
+                c = __reduce_add_sync(0xffffffffu, c);
+                __syncthreads();                 // (ncand has been read)
+                if (tid == 0) ncand = 0;
+                __syncthreads();
+                if (lane == 0) atomicAdd(&ncand, c);
+                __syncthreads();
+                if (ncand >= p.keep) {
+                    bound = u;
+                    reach = ncand;
+                }
+            }
+            __syncthreads();
+            if (tid == 0) ncand = 0;
+            __syncthreads();
+            entries(true, [&](unsigned long long k) {
+                if (k >= bound) collect(k);
+            });
+            __syncthreads();
+        }
     }
-    const int all = ncand, have = min(all, kCand);
+    const int have = ncand;
     for (int i = tid; i < have; i += kT) {
         const unsigned long long k = cand[i];
         int r = 0;
@@ -914,7 +940,7 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     }
     // settled: there is nothing outside the candidates, or it cannot reach the n-th
     const float outside = lead_n > 0 ? top_value(lead[lead_n - 1]) : INFINITY;
-    const bool settled = fine && all <= kCand && lead_n >= p.n &&
+    const bool settled = fine && lead_n >= p.n &&
                          (lead_n == p.V || (err == 0.f ? top_value(nth) >= outside
                                                        : top_value(nth) > outside + kMargin * err));
 #pragma unroll

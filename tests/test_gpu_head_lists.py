@@ -109,3 +109,23 @@ def test_one_long_list(dev):
     up = torch.arange(V).float() / 8
     for T in (2, 129):
         check_kinds([up, up.flip(0)], [V - 1, 0], T, 32, dev)
+
+
+@pytest.mark.parametrize("n", [0, 3, 32])
+def test_candidates_crowded_in_few_threads(dev, n):
+    """More large logits than are ranked at once, held by fewer threads than alternatives are kept, so that the
+    threads' best ones are no bound on them: in each of 27 of a row's 48 lists (one tile of 256 columns a part at
+    600 rows of 6,144 logits) the columns that lie 0 to 9 above a multiple of 32 are far above the rest. The 40
+    largest come in one of the last lists."""
+    V, T = 24 * 256, 600
+    v = torch.arange(V)
+    lists, lane = torch.div(v, 128, rounding_mode="floor"), v % 32
+    high = lists % 16 <= 8
+    peak = high & (lane < 10) & ~((lists % 4 == 1) & (lane == 9))
+    rng = torch.Generator().manual_seed(40)
+    row = torch.where(high, 1.0, 0.0)
+    row[peak] = 50.0 + torch.randperm(int(peak.sum()), generator=rng).float() / 256
+    best = peak & (lists == 40)
+    row[best] = 60.0 + torch.randperm(int(best.sum()), generator=rng).float() / 16
+    check_kinds([row], [int(row.argmax())], T, n, dev)
+    check_kinds([row], [7], T, n, dev)
