@@ -782,11 +782,17 @@ size_t moe_head_logprobs_workspace_bytes(int T, int V, int n);
 
 /*
  * The same outputs straight from bf16 rows x [T, H] and the bf16 head [V, H] (both 16-byte aligned,
- * H a multiple of 8 up to 8192; any T): prompt scoring without [T, V] logits in memory. The ids are
- * in the order of the logits moe_lm_head_logits computes, and the logits of the targets and of the
- * alternatives are those. A row with a logit that is not finite has no distribution. The sums over the
- * other logits take the tensor cores' own, which are off by up to their size times H / 16 * 2^-23; logits
- * from 2^30 in size on may give NaN. Calls that share a workspace must not overlap on the GPU.
+ * H a multiple of 8 up to 8192; any T): prompt scoring without [T, V] logits in memory. The logits of the
+ * targets and of the alternatives are those moe_lm_head_logits computes (64-bit sums, rounded once), and the ids
+ * are in their order wherever what is certain about the others allows it: the tensor cores' sums, by which
+ * the others are left out, are off by up to H / 16 * 2^-23 times sum_h |x_h w_vh|. With S the largest such
+ * sum of magnitudes among the row's n + 8 best, a row whose n-th logit does not lie above the others by four
+ * times that error of S is ordered by all V logits in 64 bits. A token can be missed only if its own sum of
+ * magnitudes is more than 4 S: large products that cancel beside leaders without any (moe_lm_head_logits and
+ * moe_token_logprobs order those too). The log of the sum over the others takes the tensor cores' sums: it is
+ * off by up to H / 16 * 2^-22 times their largest sum of magnitudes (a few 1e-7 in ordinary rows). A row
+ * with a logit that is not finite has no distribution; logits from 2^30 in size on may give NaN.
+ * Calls that share a workspace must not overlap on the GPU.
  */
 int moe_head_logprobs(const void *head, int V, int H, const void *x, int T, const int32_t *targets, int n,
                       float *logprob, float *entropy, int32_t *top_ids, float *top_logprobs, void *workspace,

@@ -21,9 +21,13 @@
 //
 // A tensor-core logit carries the rounding of H / 16 fp32 accumulations. That moves the log of the sum
 // of e^logit by the probability-weighted mean of those errors, a few 1e-7; it must not move an id or a
-// logit that is returned, hence the second sum. A candidate list is enough when the n-th exact logit
-// lies above the best logit outside by kMargin times the largest error seen among the row's
-// candidates, or when those errors are all zero.
+// logit that is returned, hence the second sum. The errors go by the sums of magnitudes sum_h |x_h w_vh|,
+// not by the logits: a candidate list is enough when the n-th exact logit lies above the best logit outside
+// by what the accumulations may lose of kSpread times the largest such sum among the row's candidates, and by kMargin
+// times the largest error seen among them. For N(0, 1) rows on a head of 248,320 x 3,072 that is 0.004 beside the
+// 0.05 to 0.07 that lie between the n-th and the (n + 8)-th logit (n = 32, 20), so that hardly a row
+// is left to exact_kernel. An entry outside whose magnitudes exceed those of all candidates by more than kSpread may
+// be missed: nothing here has seen it.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -49,7 +53,7 @@ constexpr int kPad = 8;                // kept beyond n, to tell whether the ord
 constexpr int kKeep = kTopMax + kPad;  // at most
 constexpr int kBins = 64;              // disjoint maxima of a row, for a bound on its keep-th largest logit
 constexpr int kMaxGroup = 8;           // 256-row blocks per launch: 74 / 8 = 9 parts, 144 of 148 CTAs busy
-constexpr float kMargin = 16.f;
+constexpr float kMargin = 16.f, kSpread = 4.f;         // see above
 constexpr int kExCluster = 8, kMaxClusters = 32;       // exact_kernel: CTAs per cluster, clusters at most
 
 struct ScoreArgs {
@@ -648,27 +652,41 @@ MOE_D void stage_row(const uint16_t *x, int H, float4 *xs) {
 }
 
 // A warp's dot product of a head row with the staged row: the products (exact in fp32) summed in
-// 64 bits in the LM head's order, rounded once
-MOE_D float exact_logit(const uint16_t *w, const float4 *xs, int H) {
+// 64 bits in the LM head's order, rounded once. size: the sum of their magnitudes.
+template <bool kSize>
+MOE_D float exact_logit(const uint16_t *w, const float4 *xs, int H, float &size) {
     const int lane = threadIdx.x & 31, nch = H / 8;
     const uint4 *wr = reinterpret_cast<const uint4 *>(w);
     double acc = 0.0;
+    float mag = 0.f;
+    auto add = [&](float p) {
+        acc += (double)p;
+        if (kSize) mag += fabsf(p);
+    };
 #pragma unroll 4
     for (int c = lane; c < nch; c += 32) {
         const uint4 q = __ldg(wr + c);
         const float4 a = xs[c], b = xs[nch + c];
-        acc += (double)(__uint_as_float(q.x << 16) * a.x);
-        acc += (double)(__uint_as_float(q.x & 0xffff0000u) * a.y);
-        acc += (double)(__uint_as_float(q.y << 16) * a.z);
-        acc += (double)(__uint_as_float(q.y & 0xffff0000u) * a.w);
-        acc += (double)(__uint_as_float(q.z << 16) * b.x);
-        acc += (double)(__uint_as_float(q.z & 0xffff0000u) * b.y);
-        acc += (double)(__uint_as_float(q.w << 16) * b.z);
-        acc += (double)(__uint_as_float(q.w & 0xffff0000u) * b.w);
+        add(__uint_as_float(q.x << 16) * a.x);
+        add(__uint_as_float(q.x & 0xffff0000u) * a.y);
+        add(__uint_as_float(q.y << 16) * a.z);
+        add(__uint_as_float(q.y & 0xffff0000u) * a.w);
+        add(__uint_as_float(q.z << 16) * b.x);
+        add(__uint_as_float(q.z & 0xffff0000u) * b.y);
+        add(__uint_as_float(q.w << 16) * b.z);
+        add(__uint_as_float(q.w & 0xffff0000u) * b.w);
     }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    for (int off = 16; off > 0; off >>= 1) {
+        acc += __shfl_xor_sync(0xffffffffu, acc, off);
+        if (kSize) mag += __shfl_xor_sync(0xffffffffu, mag, off);
+    }
+    if (kSize) size = mag;
     return (float)acc;
+}
+MOE_D float exact_logit(const uint16_t *w, const float4 *xs, int H) {
+    float none;
+    return exact_logit<false>(w, xs, H, none);
 }
 
 // ------------------------------------------------------------------ one row's parts joined
@@ -697,7 +715,7 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     constexpr int kW = kT / 32;
     extern __shared__ float4 xs[];                                  // the row (stage_row)
     __shared__ unsigned long long cand[kCand], lead[kKeep];
-    __shared__ float peaks[kMaxLists], groups[kGroups], exact[kKeep + 1];
+    __shared__ float peaks[kMaxLists], groups[kGroups], exact[kKeep + 1], sizes[kW];
     __shared__ unsigned long long bound_s;
     __shared__ int counts[kMaxLists];
     __shared__ Soft softs[kW];
@@ -854,14 +872,23 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     const int lead_n = min(have, p.keep);
     const int target = p.targets ? p.targets[row] : -1;
     const bool has_target = target >= 0 && target < p.V;
+    float widest = 0.f;                          // the largest sum of magnitudes behind a leading one
     for (int i = warp; i <= lead_n; i += kW) {
         const int id = i < lead_n ? top_index(lead[i]) : target;
         const bool in = id >= 0 && id < p.V;
-        const float l = in ? exact_logit(p.head + (size_t)id * p.H, xs, p.H) : 0.f;
+        float mine = 0.f;
+        const float l = in ? exact_logit<true>(p.head + (size_t)id * p.H, xs, p.H, mine) : 0.f;
         if (lane == 0) exact[i] = l;
+        if (i < lead_n) widest = fmaxf(widest, mine);
     }
+    if (lane == 0) sizes[warp] = widest;
     __syncthreads();
     if (warp != 0) return;
+    widest = lane < kW ? sizes[lane] : 0.f;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, off));
+    // Each of the tensor cores' H / 16 steps loses at most 2^-23 of what it holds
+    const float loss = (float)((p.H + 15) / 16) * 1.1920929e-7f;
 
     // Statistics relative to the exact logit of the leading candidate, which they leave out, with the
     // others' exact logits in place of the tensor cores'. The tensor cores' accumulation rounds towards zero:
@@ -900,10 +927,9 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
         const float d = st.m - sum.m, f = expf(d);
         const float rs = fmaf(f, st.s, -near_sum.s), rw = f * (st.w + d * st.s) - near_sum.w;     // the rest
         if (rs > 0.f) {
-            // Each of the H / 16 steps loses at most 2^-23 of the sum so far. A larger share is no share: the
-            // candidates' sums cancel, their errors have nothing to do with their size, and the rest stays.
-            const float most = (float)((p.H + 15) / 16) * 1.1920929e-7f;
-            const float rho = fabsf(gain) <= most * size && size > 0.f ? gain / size : 0.f;
+            // A share larger than the loss is no share: the candidates' sums cancel, their errors have nothing to
+            // do with their size, and the rest stays.
+            const float rho = fabsf(gain) <= loss * size && size > 0.f ? gain / size : 0.f;
             const float moved = rho * fmaf(sum.m, rs, rw);
             sum.s += rs + moved;
             sum.w += rw + moved * (1.f + rw / rs);
@@ -938,11 +964,11 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
         const unsigned who = __ballot_sync(0xffffffffu, key[h] != 0ull && rank[h] == p.n - 1);
         if (who) nth = __shfl_sync(0xffffffffu, key[h], __ffs(who) - 1);
     }
-    // settled: there is nothing outside the candidates, or it cannot reach the n-th
+    // settled: there is nothing outside the candidates, or it cannot reach the n-th (a row of zeros: no error)
     const float outside = lead_n > 0 ? top_value(lead[lead_n - 1]) : INFINITY;
+    const float margin = fmaxf(kMargin * err, kSpread * loss * widest);
     const bool settled = fine && lead_n >= p.n &&
-                         (lead_n == p.V || (err == 0.f ? top_value(nth) >= outside
-                                                       : top_value(nth) > outside + kMargin * err));
+                         (lead_n == p.V || (margin == 0.f ? top_value(nth) >= outside : top_value(nth) > outside + margin));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (key[h] != 0ull && rank[h] < p.n) {

@@ -71,7 +71,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, n:
 def head_logprobs(head: torch.Tensor, h: torch.Tensor, targets: torch.Tensor | None = None, n: int = 0,
                   stream=None) -> TokenLogprobs:
     """token_logprobs of the logits of rows h bf16 [T, H] under the head bf16 [V, H], without the
-    [T, V] logits in memory (prompt scoring): any T."""
+    [T, V] logits in memory (prompt scoring): any T. The alternatives are exact unless a token's sum_h
+    |x_h w_vh| is more than four times the largest one's among the row's n + 8 best."""
     _need(head, "head", (torch.bfloat16,))
     dev = head.device
     _need(h, "h", (torch.bfloat16,), dev)
