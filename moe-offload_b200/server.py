@@ -140,13 +140,20 @@ def _token_text(tok, i: int) -> str:
     return text if text and "\ufffd" not in text else f"token_id:{i}"
 
 
+def _token_bytes(tok, i: int) -> bytes:
+    """The bytes a token stands for; of a tokenizer that does not tell, those of a text of its own."""
+    if hasattr(tok, "decode_bytes"):
+        return tok.decode_bytes([i])
+    text = tok.decode([i])
+    return b"" if "\ufffd" in text else text.encode()
+
+
 def _logprobs_json(tok, records: list[dict], is_chat: bool, offset: int = 0, first: bool = False) -> dict:
     """The records of consecutive tokens in the response's form. Completions: offset is the first one's place in
     the text, first: a prompt's first token stands before them, without a log-probability."""
     if is_chat:
         def entry(i, lp):
-            text = _token_text(tok, i)
-            return {"token": text, "logprob": _finite(lp), "bytes": list(text.encode())}
+            return {"token": _token_text(tok, i), "logprob": _finite(lp), "bytes": list(_token_bytes(tok, i)) or None}
         return {"content": [{**entry(r["id"], r["logprob"]), "top_logprobs": [entry(*t) for t in r["top"]]}
                             for r in records]}
     tokens = [_token_text(tok, r["id"]) for r in records]

@@ -103,7 +103,11 @@ class ByteTokenizer:
         return list(text.encode("utf-8"))
 
     def decode(self, ids: Iterable[int]) -> str:
-        return bytes(i for i in ids if 0 <= i < 256).decode("utf-8", errors="replace")
+        return self.decode_bytes(ids).decode("utf-8", errors="replace")
+
+    def decode_bytes(self, ids: Iterable[int]) -> bytes:
+        """What the ids stand for before it is read as text (a token may be part of a character)."""
+        return bytes(i for i in ids if 0 <= i < 256)
 
 
 class TokenHead:
