@@ -17,6 +17,7 @@ prompt here is "role: content" lines and "assistant: ", encoded by the engine's 
 from __future__ import annotations
 
 import argparse
+import codecs
 import json
 import math
 import queue
@@ -148,19 +149,31 @@ def _token_bytes(tok, i: int) -> bytes:
     return b"" if "\ufffd" in text else text.encode()
 
 
-def _logprobs_json(tok, records: list[dict], is_chat: bool, offset: int = 0, first: bool = False) -> dict:
-    """The records of consecutive tokens in the response's form. Completions: offset is the first one's place in
-    the text, first: a prompt's first token stands before them, without a log-probability."""
+class _Places:
+    """Where in a text that starts at `at` its tokens stand, one after another: the parts of a character at that
+    character."""
+
+    def __init__(self, tok, at: int = 0):
+        self.tok, self.at = tok, at
+        self.text = codecs.getincrementaldecoder("utf-8")("replace")     # (holds back what may be part of one)
+
+    def next(self, i: int) -> int:
+        b = _token_bytes(self.tok, i)
+        new = len(self.text.decode(b))
+        here = self.at + max(0, new - len(b.decode("utf-8", errors="replace")))
+        self.at += new
+        return here
+
+
+def _logprobs_json(tok, records: list[dict], is_chat: bool, offsets: list[int], first: bool = False) -> dict:
+    """The records of consecutive tokens in the response's form. Completions: offsets are their places in the
+    text, first: a prompt's first token stands before them, without a log-probability."""
     if is_chat:
         def entry(i, lp):
             return {"token": _token_text(tok, i), "logprob": _finite(lp), "bytes": list(_token_bytes(tok, i)) or None}
         return {"content": [{**entry(r["id"], r["logprob"]), "top_logprobs": [entry(*t) for t in r["top"]]}
                             for r in records]}
     tokens = [_token_text(tok, r["id"]) for r in records]
-    offsets = []
-    for r in records:
-        offsets.append(offset)
-        offset += len(tok.decode([r["id"]]))
     out = {"tokens": tokens, "token_logprobs": [_finite(r["logprob"]) for r in records],
            "top_logprobs": [{_token_text(tok, i): _finite(lp) for i, lp in r["top"]} for r in records],
            "text_offset": offsets}
@@ -311,7 +324,7 @@ class Handler(BaseHTTPRequestHandler):
         head = tok.decode(prompt_ids) if echo else ""
         gen = srv.worker.stream(prompt_ids, max_tokens, temperature=temperature, top_p=top_p, seed=seed,
                                 timings=timings, **more)
-        told = 0
+        told, places = 0, _Places(tok, len(head))
 
         def lp_of(last: int):
             """The response's logprobs of the tokens from `told` up to `last`, with the echoed prompt's before the
@@ -319,12 +332,14 @@ class Handler(BaseHTTPRequestHandler):
             nonlocal told
             if logprobs is None:
                 return None
-            part, at, first = scored[told:last], told, echo and told == 0 and bool(prompt_ids)
+            part, first = scored[told:last], echo and told == 0 and bool(prompt_ids)
+            offsets = [places.next(r["id"]) for r in part]
             if first:
                 part = [{"id": prompt_ids[0], "logprob": math.nan, "top": []}] + prompt_scored + part
+                before = _Places(tok)
+                offsets = [before.next(i) for i in prompt_ids] + offsets
             told = last
-            start = 0 if first else len(head) + len(tok.decode(ids[:at]))
-            return _logprobs_json(tok, part, is_chat, start, first)
+            return _logprobs_json(tok, part, is_chat, offsets, first)
         if stream:
             self.send_response(200)
             self.send_header("Content-Type", "text/event-stream")

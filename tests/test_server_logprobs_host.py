@@ -60,3 +60,48 @@ def test_bytes_of_an_id_without_any(serve):
     content = chat(serve(Says([65, 298])), top_logprobs=2)
     assert content[1]["token"] == "token_id:298" and content[1]["bytes"] is None
     assert content[1]["top_logprobs"][0]["bytes"] is None and content[0]["bytes"] == [65]
+
+
+def completion(srv, **more):
+    st, data = post(srv, "/v1/completions", {"max_tokens": 40, "logprobs": 0, **more})
+    assert st == 200
+    return strict(data)["choices"][0]
+
+
+TEXT = "a\xe9b€\U0001f600.c"
+
+
+def places(text):
+    """Where in the text each byte's character stands."""
+    return [k for k, c in enumerate(text) for _ in c.encode()]
+
+
+def test_offsets_of_parts_of_a_character(serve):
+    choice = completion(serve(Says(list(TEXT.encode()))), prompt="x")
+    assert choice["text"] == TEXT and choice["logprobs"]["text_offset"] == places(TEXT)
+
+
+def test_offsets_behind_an_echoed_prompt(serve):
+    choice = completion(serve(Says(list(TEXT.encode()))), prompt="€ x\xe9", echo=True)
+    assert choice["text"] == "€ x\xe9" + TEXT and choice["logprobs"]["text_offset"] == places("€ x\xe9" + TEXT)
+
+
+@pytest.mark.parametrize("echo", [False, True])
+def test_offsets_of_a_stream(serve, echo):
+    srv = serve(Says(list(TEXT.encode())))
+    st, data = post(srv, "/v1/completions", {"prompt": "\xe9€", "max_tokens": 40, "logprobs": 0, "echo": echo, "stream": True})
+    choices = [strict(e[6:])["choices"][0] for e in data.decode().split("\n\n") if e.startswith("data: {")]
+    text = "".join(c["text"] for c in choices)
+    offsets = [o for c in choices for o in c.get("logprobs", {}).get("text_offset", [])]
+    assert text == ("\xe9€" if echo else "") + TEXT and offsets == places(text)
+
+
+def test_offsets_of_bytes_that_are_no_text(serve):
+    """Bytes that begin no character, or one that does not come: a replacement character each, and what follows
+    them stands behind those."""
+    ids = [0xe9, 0x28, 0xff, 0x80, 0x41, 298, 0x42, 0xe2, 0x82]
+    choice = completion(serve(Says(ids)), prompt="x")
+    assert choice["text"] == "�(��AB�"
+    got = choice["logprobs"]["text_offset"]
+    assert [got[ids.index(i)] for i in (0x28, 0x41, 0x42, 0xe2, 0x82)] == [1, 4, 5, 6, 6]
+    assert got == sorted(got)
