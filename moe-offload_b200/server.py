@@ -173,9 +173,15 @@ def _logprobs_json(tok, records: list[dict], is_chat: bool, offsets: list[int], 
             return {"token": _token_text(tok, i), "logprob": _finite(lp), "bytes": list(_token_bytes(tok, i)) or None}
         return {"content": [{**entry(r["id"], r["logprob"]), "top_logprobs": [entry(*t) for t in r["top"]]}
                             for r in records]}
+    def alternatives(top):
+        of: dict[str, float | None] = {}
+        for i, lp in top:
+            text = _token_text(tok, i)
+            of[f"token_id:{i}" if text in of else text] = _finite(lp)     # (ids may read alike)
+        return of
     tokens = [_token_text(tok, r["id"]) for r in records]
     out = {"tokens": tokens, "token_logprobs": [_finite(r["logprob"]) for r in records],
-           "top_logprobs": [{_token_text(tok, i): _finite(lp) for i, lp in r["top"]} for r in records],
+           "top_logprobs": [alternatives(r["top"]) for r in records],
            "text_offset": offsets}
     if first:
         out["token_logprobs"][0] = out["top_logprobs"][0] = None

@@ -105,3 +105,30 @@ def test_offsets_of_bytes_that_are_no_text(serve):
     got = choice["logprobs"]["text_offset"]
     assert [got[ids.index(i)] for i in (0x28, 0x41, 0x42, 0xe2, 0x82)] == [1, 4, 5, 6, 6]
     assert got == sorted(got)
+
+
+class OneText(Says):
+    """A vocabulary in which 66 and 67 read alike (as words with and without a leading space do in many)."""
+
+    def __init__(self, ids):
+        super().__init__(ids)
+        inner = self.tokenizer
+
+        class Tokenizer:
+            eos_token_id = inner.eos_token_id
+
+            def encode(self, text):
+                return inner.encode(text)
+
+            def decode(self, ids):
+                return inner.decode([66 if i == 67 else i for i in ids])
+
+        self.tokenizer = Tokenizer()
+
+
+def test_alternatives_of_equal_text(serve):
+    """Each alternative has its place: a second one of the same text goes by its number."""
+    choice = completion(serve(OneText([65])), prompt="x", logprobs=3)
+    assert choice["logprobs"]["top_logprobs"] == [{"A": 0.0, "B": -0.25, "token_id:67": None}]
+    choice = completion(serve(OneText([66])), prompt="x", logprobs=2)
+    assert choice["logprobs"]["top_logprobs"] == [{"B": 0.0, "token_id:67": -0.25}]
