@@ -155,6 +155,8 @@ class TokenHead:
         """h bf16 [T, H] (T <= 4) -> fp32 [T, V]. adapters (adapters.AdapterBank of K = H, N = V) with
         adapter_ids int32 [T] (device): each row's low-rank adapter is added, -1 for none."""
         _need(h, "h", (torch.bfloat16,), self.device)
+        if adapters is not None and adapter_ids is None:
+            raise ValueError("adapters need adapter_ids, one of each row")
         T = h.shape[0]
         if out is None:
             out = torch.empty((T, self.V), dtype=torch.float32, device=self.device)
