@@ -648,8 +648,11 @@ extern "C" int moe_adapter_add(const void *x, int T, int K, int N, const void *a
     const int full = 296;              // two CTAs on each of 148 SMs
     // One row a tile while reading each row's own A and B costs less than what tiles cost on top: a decode
     // batch, or up to 32 MB of them (K = 3,072, N = 768, rank 16, 30 adapters: 5.3 us against 8.6 for 100
-    // rows, 7.2 against 11.7 for 300; rank 64 of 2,048 x 2,048: 20 against 11.4 for 150). A cluster a
-    // row only where there are few (one row: 4.0 us with 8 CTAs, 64 rows: 5.0 with 1, 5.3 with 4).
+    // rows, 7.2 against 11.7 for 300; rank 64 of 2,048 x 2,048: 20 against 11.4 for 150). A batch of up to 74
+    // rows goes by rows whatever its width, where several adapters would each be a tile's: fp32 y of 248,320,
+    // 64 rows, rank 16 120 us against 167 with 8 adapters (99 with one for all), rank 64 333 against 429 (232),
+    // rank 128 638 against 1,157 (589). A cluster a row only where there are few (one row: 4.0 us with
+    // 8 CTAs, 64 rows: 5.0 with 1, 5.3 with 4).
     const bool single = T <= full / 4 || (double)T * rank * ((double)K + N) * 2 <= 32e6;
     int ctas;
     if (single) {

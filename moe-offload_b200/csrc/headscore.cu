@@ -1020,7 +1020,7 @@ __global__ void __cluster_dims__(kExCluster, 1, 1) __launch_bounds__(kExThreads)
         const int step = shares * kExCluster * kExWarps;
         for (int v = (share * kExCluster + rank) * kExWarps + warp; v < p.V; v += step) {
             const unsigned long long k = top_key(exact_logit(p.head + (size_t)v * p.H, xs, p.H), v);
-            list = top_insert(list, k, 1u);
+            list = top_insert(list, k);
         }
         lists[warp][lane] = list;
         __syncthreads();

@@ -39,9 +39,7 @@ int moe_prefill_experts_ex(const void *x, int T, int H, int I, int E, int K, con
 // xn[t] = x[t] * 2^-k(t), the per-row power-of-two RMS normalisation (prefill.cu)
 int moe_pow2_rows_launch(const void *x, int T, int H, void *xn, void *stream);
 
-// Log-probabilities of rows of fp32 logits (logprobs.cu): the launch, and the argument checks that
-// it shares with the form that starts from hidden rows (headscore.cu).
-int moe_token_logprobs_launch(const float *logits, int T, int V, const int32_t *targets, int n, float *logprob,
-                              float *entropy, int32_t *top_ids, float *top_logprobs, void *stream);
+// Argument checks that the log-probabilities of logits in memory (logprobs.cu) and from hidden rows
+// (headscore.cu) share.
 int moe_logprobs_check(const char *who, int T, int V, const int32_t *targets, int n, const float *logprob,
                        const float *entropy, const int32_t *top_ids, const float *top_logprobs);

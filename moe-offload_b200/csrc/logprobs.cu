@@ -327,10 +327,8 @@ __global__ void __launch_bounds__(kT) logprobs_kernel(LogprobArgs p) {
     }
 }
 
-}  // namespace
-
-int moe_token_logprobs_launch(const float *logits, int T, int V, const int32_t *targets, int n, float *logprob,
-                              float *entropy, int32_t *top_ids, float *top_logprobs, void *stream) {
+int launch_logprobs(const LogprobArgs &p, cudaStream_t stream) {
+    const int T = p.T, V = p.V;
     // A CTA's work behind the pass over its elements is a chain of some 5,000 cycles, whatever it has read. So:
     // a cluster only as far as the rows leave SMs free (T = 64, V = 248,320: 21.5 us with 4 CTAs a row, 25.6
     // with 2, 29.7 with 8; T = 1: 10.2 with 8, 23.6 with 1), and fewer threads for many short rows
@@ -347,18 +345,19 @@ int moe_token_logprobs_launch(const float *logits, int T, int V, const int32_t *
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)T * (unsigned)parts);
     cfg.blockDim = dim3((unsigned)threads);
-    cfg.stream = as_stream(stream);
+    cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)parts;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;            // (a CTA alone is a cluster of one)
-    const LogprobArgs p{logits, T, V, n, targets, logprob, entropy, top_ids, top_logprobs};
     auto kern = threads == 512 ? logprobs_kernel<512> : threads == 256 ? logprobs_kernel<256> : logprobs_kernel<128>;
     MOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
     return MOE_OK;
 }
+
+}  // namespace
 
 int moe_logprobs_check(const char *who, int T, int V, const int32_t *targets, int n, const float *logprob,
                        const float *entropy, const int32_t *top_ids, const float *top_logprobs) {
@@ -378,5 +377,6 @@ extern "C" int moe_token_logprobs(const float *logits, int T, int V, const int32
         return rc;
     if (!logits || (reinterpret_cast<uintptr_t>(logits) & 3))
         return moe_set_error(MOE_EINVAL, "token logprobs: logits must be 4-byte aligned and not null");
-    return moe_token_logprobs_launch(logits, T, V, targets, n, logprob, entropy, top_ids, top_logprobs, stream);
+    return launch_logprobs(LogprobArgs{logits, T, V, n, targets, logprob, entropy, top_ids, top_logprobs},
+                           as_stream(stream));
 }

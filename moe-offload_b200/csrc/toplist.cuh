@@ -89,7 +89,7 @@ MOE_D SoftRun run_none() { return SoftRun{-INFINITY, 0.f, 0.f, 0.f}; }
 template <int kN>
 MOE_D void run_add(SoftRun &a, const float (&v)[kN], float top) {
     if (top > a.m && !(top <= a.r + kRunSpan && a.m > -INFINITY)) {
-        const float d = fmaxf(a.r - top, kSoftFar), f = a.m > -INFINITY ? fast_exp(d) : 1.f;
+        const float d = fmaxf(a.r - top, kSoftFar), f = a.m > -INFINITY ? expf(d) : 1.f;
         a.w = f * (a.w + d * a.s);
         a.s *= f;                                // (nothing in the sums yet: 0, or NaN)
         a.r = top;
@@ -133,16 +133,9 @@ MOE_D unsigned long long top_merge(unsigned long long a, unsigned long long b) {
     for (int off = 16; off > 0; off >>= 1) a = top_cmpx(a, off, (lane & off) == 0);
     return a;
 }
-// inserts the keys of the lanes in `who` (a warp-uniform mask) into a sorted list, one after another
-MOE_D unsigned long long top_insert(unsigned long long list, unsigned long long key, unsigned who) {
-    const int lane = threadIdx.x & 31;
-    while (who) {
-        const int src = __ffs(who) - 1;
-        who &= who - 1;
-        const unsigned long long k = __shfl_sync(0xffffffffu, key, src);
-        const unsigned long long up = __shfl_up_sync(0xffffffffu, list, 1);
-        // entries above k stay, the others move down by one, k takes the gap
-        if (list < k) list = (lane == 0 || up > k) ? k : up;
-    }
-    return list;
+// inserts a key that all lanes hold into a sorted list
+MOE_D unsigned long long top_insert(unsigned long long list, unsigned long long key) {
+    const unsigned long long up = __shfl_up_sync(0xffffffffu, list, 1);
+    // entries above the key stay, the others move down by one, the key takes the gap
+    return list > key ? list : ((threadIdx.x & 31) == 0 || up > key) ? key : up;
 }
