@@ -708,6 +708,67 @@ struct FinishArgs {
     int *redo;                         // [0] count, counters of exact_kernel, (row, bits of m, bits of lse - m) ..
 };
 
+// Candidates where more than kCand entries reach tau: those above a bound on (value, index). Out of line: rows of
+// ties (a padded batch) and lists whose large entries lie in few places need it.
+template <int kT>
+__device__ __noinline__ void recollect(const uint2 *lists, const int *counts, int nlists, float tau, int keep,
+                                       unsigned long long *cand, int *ncand, unsigned long long *shared_bound) {
+    constexpr int kW = kT / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto entries = [&](auto &&f) {
+        for (int l = warp; l < nlists; l += kW)
+#pragma unroll
+            for (int i = 0; i < kSlots / 32; ++i) {
+                const uint2 e = lane + 32 * i < counts[l] ? lists[((size_t)l * kSlots + lane + 32 * i) * kM]
+                                                          : make_uint2(0xff800000u, 0u);           // -inf
+                const float value = __uint_as_float(e.x);
+                if (value >= tau && value > -INFINITY) f(top_key(value, (int)e.y));
+            }
+    };
+    auto collect = [&](unsigned long long bound) {
+        __syncthreads();                         // (ncand has been read)
+        if (tid == 0) *ncand = 0;
+        __syncthreads();
+        entries([&](unsigned long long k) {
+            if (k < bound) return;
+            const int at = atomicAdd(ncand, 1);
+            if (at < kCand) cand[at] = k;
+        });
+        __syncthreads();
+    };
+    // the keep-th largest of the threads' best entries
+    unsigned long long best = 0ull;
+    entries([&](unsigned long long k) { best = k > best ? k : best; });
+    __syncthreads();
+    cand[tid] = best;
+    __syncthreads();
+    int r = 0;
+    for (int j = 0; j < kT; ++j) r += (cand[j] > best || (cand[j] == best && j < tid)) ? 1 : 0;
+    if (r == keep - 1) *shared_bound = best;
+    __syncthreads();
+    collect(*shared_bound);
+    if (*ncand <= kCand) return;
+    // crowded in a few threads: a bound bit by bit, which keep to kCand keys reach (they differ)
+    unsigned long long bound = 0ull;
+    int reach = 0;
+    for (int bit = 63; bit >= 0 && !(reach >= keep && reach <= kCand); --bit) {
+        const unsigned long long u = bound | (1ull << bit);
+        int c = 0;
+        entries([&](unsigned long long k) { c += k >= u ? 1 : 0; });
+        c = __reduce_add_sync(0xffffffffu, c);
+        __syncthreads();
+        if (tid == 0) *ncand = 0;
+        __syncthreads();
+        if (lane == 0) atomicAdd(ncand, c);
+        __syncthreads();
+        if (*ncand >= keep) {
+            bound = u;
+            reach = *ncand;
+        }
+    }
+    collect(bound);
+}
+
 // kT: 512 threads for few rows (latency), 128 for many (the rows' own instructions are the bound then:
 // 98 us for 2,048 rows, 116 with 512)
 template <int kT>
@@ -791,73 +852,27 @@ __global__ void __launch_bounds__(kT) finish_kernel(FinishArgs p) {
     const float tau = tau_s;
     const bool one_round = nlists <= 2 * kW;                         // held still has all entries
     // every entry that may reach tau
-    auto entries = [&](bool again, auto &&f) {
-        for (int l = warp; l < nlists; l += 2 * kW) {
-            if (by_list || !one_round || again) {
-                const bool a = !by_list || peaks[l] >= tau;
-                const bool b = l + kW < nlists && (!by_list || peaks[l + kW] >= tau);
-                if (!a && !b) continue;
-                load_list(a ? l : nlists, held[0]);
-                load_list(b ? l + kW : nlists, held[1]);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    const float value = __uint_as_float(held[h][i].x);
-                    if (value >= tau && value > -INFINITY) f(top_key(value, (int)held[h][i].y));
-                }
+    for (int l = warp; l < nlists; l += 2 * kW) {
+        if (by_list || !one_round) {
+            const bool a = !by_list || peaks[l] >= tau;
+            const bool b = l + kW < nlists && (!by_list || peaks[l + kW] >= tau);
+            if (!a && !b) continue;
+            load_list(a ? l : nlists, held[0]);
+            load_list(b ? l + kW : nlists, held[1]);
         }
-    };
-    auto collect = [&](unsigned long long k) {
-        const int at = atomicAdd(&ncand, 1);
-        if (at < kCand) cand[at] = k;
-    };
-    entries(false, collect);
-    __syncthreads();
-    if (ncand > kCand) {                         // ties at tau: the bound again, on (value, index) of each thread's best
-        unsigned long long best = 0ull;
-        entries(true, [&](unsigned long long k) { best = k > best ? k : best; });
-        __syncthreads();
-        cand[tid] = best;
-        if (tid == 0) ncand = 0;
-        __syncthreads();
-        int r = 0;
-        for (int j = 0; j < kT; ++j) r += (cand[j] > best || (cand[j] == best && j < tid)) ? 1 : 0;
-        if (r == p.keep - 1) bound_s = best;
-        __syncthreads();
-        unsigned long long bound = bound_s;
-        entries(true, [&](unsigned long long k) {
-            if (k >= bound) collect(k);
-        });
-        __syncthreads();
-        if (ncand > kCand) {                     // crowded in a few threads: a bound bit by bit (keys differ)
-            bound = 0ull;
-            int reach = 0;
-            for (int bit = 63; bit >= 0 && !(reach >= p.keep && reach <= kCand); --bit) {
-                const unsigned long long u = bound | (1ull << bit);
-                int c = 0;
-                entries(true, [&](unsigned long long k) { c += k >= u ? 1 : 0; });
-                c = __reduce_add_sync(0xffffffffu, c);
-                __syncthreads();                 // (ncand has been read)
-                if (tid == 0) ncand = 0;
-                __syncthreads();
-                if (lane == 0) atomicAdd(&ncand, c);
-                __syncthreads();
-                if (ncand >= p.keep) {
-                    bound = u;
-                    reach = ncand;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const float value = __uint_as_float(held[h][i].x);
+                if (value >= tau && value > -INFINITY) {
+                    const int at = atomicAdd(&ncand, 1);
+                    if (at < kCand) cand[at] = top_key(value, (int)held[h][i].y);
                 }
             }
-            __syncthreads();
-            if (tid == 0) ncand = 0;
-            __syncthreads();
-            entries(true, [&](unsigned long long k) {
-                if (k >= bound) collect(k);
-            });
-            __syncthreads();
-        }
     }
+    __syncthreads();
+    if (ncand > kCand) recollect<kT>(lists, counts, nlists, tau, p.keep, cand, &ncand, &bound_s);
     const int have = ncand;
     for (int i = tid; i < have; i += kT) {
         const unsigned long long k = cand[i];
