@@ -16,8 +16,10 @@
 //   exact_kernel   rows whose order the candidates do not settle (near-equal logits, values that are not
 //                  finite): all V logits in 64 bits. It reads the rows' number and ends when there are none.
 //
-// B200, head 248,320 x 3,072: one row 242 us (0.98 of the copy rate), 256 rows 343 us, 2,048 rows 2.25 to 2.7 ms by
-// the power limit (2.20 ms at the sustained rate of the tensor cores).
+// B200, head 248,320 x 3,072, as graphs: one row 242 to 250 us by the box (0.95 to 0.98 of the copy rate), 256 rows
+// 337 to 360 us, 2,048 rows 2.25 to 2.7 ms by the power limit (2.20 ms at the sustained rate of the tensor cores).
+// With the upper 40 % of the ids 3.3 higher 264 us, 471 us and 2.6 ms; rising by 40 from the first id to the last,
+// where every tile fills the lists, 279 us, 1.56 ms and 5.2 ms.
 //
 // A tensor-core logit carries the rounding of H / 16 fp32 accumulations. That moves the log of the sum
 // of e^logit by the probability-weighted mean of those errors, a few 1e-7; it must not move an id or a
